@@ -587,6 +587,77 @@ LT_API size_t lt_sample_workspace_size(int V);
 LT_API int lt_sample(lt_ctx* ctx, const float* logits, int V, lt_sample_params* params, int* out_tok, int* hist,
                      int* count, int cap, void* ws, size_t ws_bytes);
 
+/* ---- a paged KV cache and speculative decoding (no reference counterparts) ---------------
+ * One launch serves a batch of chunks: B sequences with their new tokens (a prompt's next chunk, a
+ * drafted continuation, or one token) packed into T rows.  Rows q_start[b] .. q_start[b+1]-1 are
+ * sequence b's (q_start [B+1] ascending from 0, device ints; a sequence may have none), its token i at
+ * position len[b] + i, where len[b] (device) counts the positions cached before the chunk.  Rows past
+ * q_start[B] are neither read nor written.  The entries below only read q_start and len (but for
+ * lt_len_add_rows and lt_verify_drafts' len), so that launches can be captured and replayed.
+ *
+ * The cache of one layer is two pools of pages, [n_pages][nkv][page][hd] each: position t of sequence b
+ * is slot t % page of page table[b*table_stride + t/page], and a KV head's rows of a page lie one after
+ * the other.  Sequences may share pages that they only read.  A table entry is used only for positions
+ * that a call writes or attends.  The descriptor is a host struct, read during the call. */
+typedef struct lt_paged_kv {
+  void* kc;               /* pools, fp16 or fp32 per kv_dtype, 16-byte aligned */
+  void* vc;
+  const int* table;       /* device, page ids of B sequences */
+  int table_stride;       /* entries a sequence: it holds at most table_stride*page positions (2^30) */
+  int n_pages, page;      /* page: positions a page, a power of two */
+  int nkv, hd;            /* hd a multiple of 8, at most 256 */
+  int kv_dtype;
+} lt_paged_kv;
+
+/* RoPE and the append of the T rows of q|k|v (row_stride floats apart): the rotated q heads to q_out
+ * (rows q_stride floats apart; q_out may be qkv itself with q_stride == row_stride), the rotated k and
+ * the v to the cache.  The values of lt_rope_append_batch, bit for bit (the angle is the binary32 product
+ * of the position and freqs[j]); qkv's own k and v are left as they are.  A row whose position lies past
+ * the table's row, or in a page outside the pool, is not stored and sets *err = 1 (device int, may be
+ * null); its q is written all the same. */
+LT_API int lt_rope_append_paged(lt_ctx* ctx, const float* qkv, int row_stride, float* q_out, int q_stride, int T,
+                                const int* q_start, const int* len, int B, int nh, const float* freqs,
+                                const lt_paged_kv* kv, int* err);
+
+/* Attention of the T rows (q: nh heads of hd, rows q_stride floats apart) over the paged cache: token i of
+ * sequence b attends positions 0 .. len[b]+i, of them the last `window` where window > 0; the chunk's own
+ * rows are in the cache already.  out [T][nh*hd] fp32 = softmax(scale q.k) v, with scores, statistics and
+ * sums in fp32 or more.  What lies in masked places (any value, infinities and NaN among them) has no
+ * effect.  A position in a page outside the pool reads as a row of zeros, and rows past the table's row
+ * attend what the table holds; both set *err = 1 (device int, may be null).
+ * max_q and max_len are the host's bounds on a sequence's rows and on len[b] plus them (0: not known); they
+ * choose between kernels and splits, and results are right whatever they say.  ws holds
+ * lt_attn_paged_workspace_size(...) bytes for the same arguments, 16-byte aligned (may be null for 0). */
+LT_API int lt_attn_paged(lt_ctx* ctx, const float* q, int q_stride, int T, const int* q_start, const int* len, int B,
+                         int nh, const lt_paged_kv* kv, float* out, float scale, int window, int max_q, int max_len,
+                         void* ws, size_t ws_bytes, int* err);
+LT_API size_t lt_attn_paged_workspace_size(int T, int B, int nh, const lt_paged_kv* kv, int max_q, int max_len);
+
+/* len[b] += q_start[b+1] - q_start[b] for every sequence, at most maxt: after the last layer's attention of
+ * a chunk that needs no verification. */
+LT_API int lt_len_add_rows(lt_ctx* ctx, int* len, const int* q_start, int B, int maxt);
+
+/* Verification of drafted tokens, under lt_sample's distributions (params [B], device: temperature, top_k
+ * and top_p of each sequence).  toks [T] are the chunk's tokens as they were fed to the target, rows as
+ * above: its row r gave logits [T][V], and the draft that follows row r is toks[r+1] (a sequence of n rows
+ * has n - 1 drafts).  draft_logits [T][V] are the logits each draft was drawn from under the same params,
+ * in the row before it (a sequence's last row is not read); null: the drafts were not drawn (looked up in
+ * the text, or greedy), a distribution with all its mass on the draft.
+ * With P and Q the two distributions of row r and x its draft, x is accepted when u[r] * Q(x) < P(x).  After
+ * the accepted ones comes one token more, drawn with u of the sequence's last row: from max(P - Q, 0) of the
+ * first row whose draft was not accepted (from P where nothing is left), or from P of the last row; it is
+ * the first candidate in rank order whose running sum exceeds u times the whole.  u [T] device, in [0, 1);
+ * null: u of row i of the sequence is Philox4x32-10's with counter params[b].counter + i (as lt_sample's),
+ * and the counter advances by the sequence's rows.  Weights and sums are binary64.
+ * out_tok [T]: a sequence's n_out[b] tokens from its first row on, then -1; n_out [B] (0 for a sequence
+ * without rows).  len (may be null): len[b] += n_out[b], the chunk's rows that stay in the cache.
+ * T <= 32767, V <= 262144.  ws holds lt_verify_drafts_workspace_size(T, V, draft_logits != NULL) bytes,
+ * 8-byte aligned (0: the sizes are refused, or T is 0). */
+LT_API int lt_verify_drafts(lt_ctx* ctx, const float* logits, const float* draft_logits, const int* toks,
+                            const int* q_start, const float* u, lt_sample_params* params, int B, int T, int V,
+                            int* out_tok, int* n_out, int* len, void* ws, size_t ws_bytes);
+LT_API size_t lt_verify_drafts_workspace_size(int T, int V, int drafter);
+
 /* ---- numerics self-check (no reference counterpart: a diagnostic of this build) ----
  * Runs on the device and writes 4 counters to host memory: out[0] = non-NaN binary32
  * patterns whose hardware fp16 conversion (the quantizer's scale) differs from

@@ -22,6 +22,14 @@ LT_SAMPLE_MAX_K = 1024
 LT_MULTI_STORE, LT_MULTI_RESID, LT_MULTI_SILU = 0, 1, 2
 
 _P = c_void_p
+
+
+class PagedKvDesc(ctypes.Structure):
+    """lt_paged_kv: one layer's paged cache (a host struct, read during the call)."""
+    _fields_ = [("kc", c_void_p), ("vc", c_void_p), ("table", c_void_p), ("table_stride", c_int), ("n_pages", c_int),
+                ("page", c_int), ("nkv", c_int), ("hd", c_int), ("kv_dtype", c_int)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "lt_version": (c_int, []),
@@ -124,6 +132,14 @@ _SIGS = {
     "lt_attn_prefill_end": (c_int, [_P, _P, c_int, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_float, c_int,
                                     c_int, c_int, _P, c_size_t, c_int]),
     "lt_embed_q8_batch": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, _P]),
+    "lt_rope_append_paged": (c_int, [_P, _P, c_int, _P, c_int, c_int, _P, _P, c_int, c_int, _P,
+                                     POINTER(PagedKvDesc), _P]),
+    "lt_attn_paged": (c_int, [_P, _P, c_int, c_int, _P, _P, c_int, c_int, POINTER(PagedKvDesc), _P, c_float, c_int,
+                              c_int, c_int, _P, c_size_t, _P]),
+    "lt_attn_paged_workspace_size": (c_size_t, [c_int, c_int, c_int, POINTER(PagedKvDesc), c_int, c_int]),
+    "lt_len_add_rows": (c_int, [_P, _P, _P, c_int, c_int]),
+    "lt_verify_drafts": (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, _P, _P, _P, _P, c_size_t]),
+    "lt_verify_drafts_workspace_size": (c_size_t, [c_int, c_int, c_int]),
     "lt_selftest_numerics": (c_int, [_P, _P]),
     "lt_selftest_attn_numerics": (c_int, [_P, _P]),
     "lt_graph_begin": (c_int, [_P]),

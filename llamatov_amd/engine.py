@@ -408,6 +408,128 @@ class KVCache:
 
 
 # ----------------------------------------------------------------------------------
+# Paged KV cache and speculative decoding: batches of chunks of new tokens
+# ----------------------------------------------------------------------------------
+class PagedKV:
+    """One layer's paged cache as the launches take it: K and V pools [n_pages][nkv][page][hd] and the
+    table of page ids, int32 [sequences][pages a sequence] (lt_paged_kv; no reference counterpart, its
+    DeviceKVCache holds one sequence).  The tensors stay the caller's."""
+    __slots__ = ("k", "v", "table", "desc")
+
+    def __init__(self, k: DevTensor, v: DevTensor, table: DevTensor, kv_dtype: int):
+        if len(k.shape) != 4 or k.shape != v.shape:
+            raise ValueError(f"PagedKV: pools {k.shape} and {v.shape} are not both [n_pages, nkv, page, hd]")
+        if len(table.shape) != 2 or table.dtype != np.int32:
+            raise ValueError(f"PagedKV: table {table.shape} {table.dtype} is not int32 [sequences, pages]")
+        want = {LT_KV_F16: 2, LT_KV_F32: 4}.get(kv_dtype)
+        if want is None or k.dtype.itemsize != want or v.dtype.itemsize != want:
+            raise ValueError(f"PagedKV: pools of {k.dtype} and {v.dtype} for kv_dtype {kv_dtype}")
+        n_pages, nkv, page, hd = k.shape
+        self.k, self.v, self.table = k, v, table
+        self.desc = _lib.PagedKvDesc(k.ptr, v.ptr, table.ptr, table.shape[1], n_pages, page, nkv, hd, kv_dtype)
+
+
+class PagedKVCache:
+    """The paged caches of a model's layers, one table and one length array for all of them, and the host's
+    account of pages: reserve() gives a sequence the pages of its next positions, release() takes them back.
+    The device lengths count the positions cached before a chunk; the launches do not change them
+    (lt_len_add_rows, lt_verify_drafts and set_lengths do)."""
+
+    def __init__(self, n_layers: int, n_pages: int, page: int, nkv: int, hd: int, max_seqs: int, max_pages: int,
+                 kv_dtype: int = LT_KV_F16, dev: Device | None = None):
+        if page <= 0 or page & (page - 1):
+            raise ValueError(f"PagedKVCache: page={page} (a power of two)")
+        if min(n_layers, n_pages, nkv, hd, max_seqs, max_pages) <= 0:
+            raise ValueError("PagedKVCache: sizes must be positive")
+        self.dev = dev or get_device()
+        self.page, self.n_pages, self.max_seqs, self.max_pages = int(page), int(n_pages), int(max_seqs), int(max_pages)
+        dt = np.uint16 if kv_dtype == LT_KV_F16 else np.float32
+        self.table = DevTensor.from_host(np.full((max_seqs, max_pages), -1, np.int32), self.dev)
+        self.lens = DevTensor.zeros((max_seqs,), np.int32, self.dev)
+        shape = (n_pages, nkv, page, hd)
+        self.layers = [PagedKV(DevTensor.empty(shape, dt, self.dev), DevTensor.empty(shape, dt, self.dev), self.table,
+                               kv_dtype) for _ in range(n_layers)]
+        self.free_pages = list(range(n_pages))[::-1]
+        self.pages: list[list[int]] = [[] for _ in range(max_seqs)]
+
+    def reserve(self, b: int, positions: int) -> None:
+        """Pages for sequence b's first `positions` positions; its table row on the device follows."""
+        need = -(-int(positions) // self.page)
+        more = need - len(self.pages[b])
+        if need > self.max_pages:
+            raise ValueError(f"sequence {b}: {positions} positions take {need} pages (at most {self.max_pages})")
+        if more > len(self.free_pages):
+            raise ValueError(f"sequence {b}: {more} pages needed, {len(self.free_pages)} free")
+        if more <= 0:
+            return
+        self.pages[b] += [self.free_pages.pop() for _ in range(more)]
+        self._push_row(b)
+
+    def release(self, b: int) -> None:
+        """Sequence b's pages go back to the pool; its length becomes 0."""
+        self.free_pages += self.pages[b][::-1]
+        self.pages[b] = []
+        self._push_row(b)
+        self.dev.h2d(self.lens.ptr + 4 * b, np.zeros(1, np.int32))
+
+    def _push_row(self, b: int) -> None:
+        row = np.full(self.max_pages, -1, np.int32)
+        row[:len(self.pages[b])] = self.pages[b]
+        self.dev.h2d(self.table.ptr + 4 * b * self.max_pages, row)
+
+    def set_lengths(self, lens) -> None:
+        self.lens.upload(np.asarray(lens, np.int32))
+
+    def lengths(self) -> list[int]:
+        return [int(n) for n in self.lens.to_host()]
+
+    def free(self) -> None:
+        self.dev.sync()
+        for L in self.layers:
+            L.k.free()
+            L.v.free()
+        self.table.free()
+        self.lens.free()
+
+
+def rope_append_paged_into(qkv: DevTensor, q_out: DevTensor, q_start: DevTensor, lens: DevTensor, nh: int,
+                           freqs: DevTensor, kv: PagedKV, err: DevTensor | None = None) -> DevTensor:
+    """RoPE of q|k|v rows [T, width] at each sequence's positions, rotated q into q_out [T, ...], k and v into
+    the paged cache (lt_rope_append_paged)."""
+    call("lt_rope_append_paged", qkv.dev.handle, qkv.ptr, qkv.shape[1], q_out.ptr, q_out.shape[1], qkv.shape[0],
+         q_start.ptr, lens.ptr, q_start.n - 1, nh, freqs.ptr, kv.desc, _vp(err))
+    return q_out
+
+
+def attn_paged_workspace_size(T: int, B: int, nh: int, kv: PagedKV, max_q: int = 0, max_len: int = 0) -> int:
+    return int(_lib.raw("lt_attn_paged_workspace_size")(T, B, nh, kv.desc, max_q, max_len))
+
+
+def attn_paged_into(q: DevTensor, q_start: DevTensor, lens: DevTensor, kv: PagedKV, nh: int, scale: float,
+                    out: DevTensor, max_q: int = 0, max_len: int = 0, window: int = 0, ws: DevTensor | None = None,
+                    err: DevTensor | None = None) -> DevTensor:
+    """Attention of the rows of q [T, at least nh*hd] over the paged cache into out [T, nh*hd] (lt_attn_paged)."""
+    call("lt_attn_paged", q.dev.handle, q.ptr, q.shape[1], q.shape[0], q_start.ptr, lens.ptr, q_start.n - 1, nh, kv.desc,
+         out.ptr, scale, window, max_q, max_len, ws.ptr if ws is not None else None,
+         ws.nbytes if ws is not None else 0, _vp(err))
+    return out
+
+
+def verify_drafts_workspace_size(T: int, V: int, drafter: bool) -> int:
+    return int(_lib.raw("lt_verify_drafts_workspace_size")(T, V, int(drafter)))
+
+
+def verify_drafts_into(logits: DevTensor, toks: DevTensor, q_start: DevTensor, u: DevTensor | None, params: DevTensor,
+                       out_tok: DevTensor, n_out: DevTensor, ws: DevTensor, draft_logits: DevTensor | None = None,
+                       lens: DevTensor | None = None) -> DevTensor:
+    """Accept or reject the drafts of a batch of chunks against logits [T, V] and draw each sequence's next token
+    (lt_verify_drafts); u None: the numbers come from each sequence's sampling state."""
+    call("lt_verify_drafts", logits.dev.handle, logits.ptr, _vp(draft_logits), toks.ptr, q_start.ptr, _vp(u), params.ptr,
+         q_start.n - 1, logits.shape[0], logits.shape[1], out_tok.ptr, n_out.ptr, _vp(lens), ws.ptr, ws.nbytes)
+    return out_tok
+
+
+# ----------------------------------------------------------------------------------
 # Production profile (a frozen config object instead of the reference's env flags)
 # ----------------------------------------------------------------------------------
 @dataclass(frozen=True)
