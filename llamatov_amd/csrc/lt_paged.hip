@@ -1,5 +1,4 @@
-// lt_paged.hip -- a packed batch of chunks over a paged KV cache: RoPE and the append of the new tokens, and
-// their attention.
+// lt_paged.hip -- the paged KV cache: RoPE and the append of a packed batch of chunks, and the lengths.
 #include "lt_paged.h"
 #include "lt_q8_device.h"
 
@@ -50,70 +49,6 @@ __global__ __launch_bounds__(256) void k_rope_append_paged(const float* __restri
   }
 }
 
-struct AttnArgs {
-  const float* q;
-  int q_stride;
-  const int* q_start;
-  const int* len;
-  int B, T, nh;
-  PagedKv C;
-  float* out;
-  float scale;
-  int window;
-  int* err;
-};
-
-// One wave a row and head: lane j scores key j of each 64, the softmax running over the 64s; lane d then sums the
-// values' dimension d.
-template <bool kF16>
-__global__ __launch_bounds__(64) void k_attn_paged_rows(AttnArgs A) {
-  const PagedKv& C = A.C;
-  const int r = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, hd = C.hd;
-  const int b = seq_of_row(A.q_start, A.B, r);
-  if (b < 0) return;
-  const int h = head / (A.nh / C.nkv);
-  const int cap = C.stride << C.shift;
-  const int past = A.len[b] < 0 ? 0 : A.len[b] < cap ? A.len[b] : cap;
-  const int pos = past + (r - A.q_start[b]);
-  const int end = pos < cap ? pos + 1 : cap;
-  const int lo = A.window > 0 && pos + 1 > A.window ? pos + 1 - A.window : 0;
-  if (pos >= cap && A.err && lane == 0) *A.err = 1;
-  const float* q = A.q + (size_t)r * A.q_stride + (size_t)head * hd;
-  auto at = [&](const void* c, size_t i) { return kF16 ? lt_h2f(((const uint16_t*)c)[i]) : ((const float*)c)[i]; };
-  float m = -__builtin_inff(), z = 0.0f, o[4] = {0, 0, 0, 0};
-  for (int k0 = lo; k0 < end; k0 += 64) {
-    const int key = k0 + lane;
-    int pg = key < end ? page_of(C, b, key) : 0;
-    if (pg < 0 && A.err) *A.err = 1;
-    float s = -__builtin_inff();
-    if (key < end) {
-      s = 0.0f;
-      if (pg >= 0)
-        for (int d = 0; d < hd; d++) s = fmaf(q[d], at(C.kc, paged_row(C, pg, h, key) + d), s);
-      s *= A.scale;
-    }
-    float mt = s;
-    for (int x = 32; x; x >>= 1) mt = fmaxf(mt, __shfl_xor(mt, x, 64));
-    const float mn = fmaxf(m, mt), mu = mn == -__builtin_inff() ? 0.0f : mn;
-    const float a = expf(m - mu), p = expf(s - mu);
-    float zt = p;
-    for (int x = 32; x; x >>= 1) zt += __shfl_xor(zt, x, 64);
-    z = z * a + zt;
-    m = mn;
-    for (int i = 0; i < 4; i++) o[i] *= a;
-    for (int j = 0; j < 64 && k0 + j < end; j++) {
-      const int pj = __shfl(pg, j, 64);
-      const float w = __shfl(p, j, 64);
-      if (pj < 0) continue;
-      for (int i = 0; i < 4; i++)
-        if (lane + 64 * i < hd) o[i] = fmaf(w, at(C.vc, paged_row(C, pj, h, k0 + j) + lane + 64 * i), o[i]);
-    }
-  }
-  for (int i = 0; i < 4; i++)
-    if (lane + 64 * i < hd)
-      A.out[((size_t)r * A.nh + head) * hd + lane + 64 * i] = end > lo ? o[i] / z : 0.0f;
-}
-
 // each length advanced by its sequence's rows (clamped to maxt)
 __global__ __launch_bounds__(256) void k_len_add_rows(int* __restrict__ len, const int* __restrict__ q_start, int B,
                                                       int maxt) {
@@ -162,29 +97,6 @@ int lt_rope_append_paged(lt_ctx* ctx, const float* qkv, int row_stride, float* q
   auto kernel = kv->kv_dtype == LT_KV_F16 ? k_rope_append_paged<true> : k_rope_append_paged<false>;
   kernel<<<T, 256, 0, ctx->stream>>>(qkv, row_stride, q_out, q_stride, q_start, len, B, nh, freqs, C, err);
   return lt_check_launch("k_rope_append_paged");
-}
-
-size_t lt_attn_paged_workspace_size(int T, int B, int nh, const lt_paged_kv* kv, int max_q, int max_len) {
-  return 0;
-}
-
-int lt_attn_paged(lt_ctx* ctx, const float* q, int q_stride, int T, const int* q_start, const int* len, int B, int nh,
-                  const lt_paged_kv* kv, float* out, float scale, int window, int max_q, int max_len, void* ws,
-                  size_t ws_bytes, int* err) {
-  const char* fn = "lt_attn_paged";
-  LT_REQUIRE(q && out && q_start && len, "%s: null argument", fn);
-  PagedKv C;
-  if (int rc = lt_paged_check(fn, kv, nh, &C)) return rc;
-  LT_REQUIRE(T >= 0 && B > 0 && q_stride >= (long long)nh * C.hd, "%s: T=%d B=%d q_stride=%d (at least %d)", fn, T, B,
-             q_stride, nh * C.hd);
-  LT_REQUIRE(window >= 0 && max_q >= 0 && max_len >= 0, "%s: window=%d max_q=%d max_len=%d", fn, window, max_q, max_len);
-  LT_REQUIRE(ctx, "%s: null ctx", fn);
-  if (T == 0) return LT_OK;
-  const LtDeviceGuard guard(ctx);
-  const AttnArgs A = {q, q_stride, q_start, len, B, T, nh, C, out, scale, window, err};
-  auto kernel = kv->kv_dtype == LT_KV_F16 ? k_attn_paged_rows<true> : k_attn_paged_rows<false>;
-  kernel<<<dim3(T, nh), 64, 0, ctx->stream>>>(A);
-  return lt_check_launch("k_attn_paged_rows");
 }
 
 int lt_len_add_rows(lt_ctx* ctx, int* len, const int* q_start, int B, int maxt) {

@@ -167,6 +167,15 @@ def test_attention_windows(gpu, window, kv):
         b.free()
 
 
+def test_attention_split_windows(gpu):
+    """Windows over long contexts: the workspace of the whole context serves every window."""
+    b = Batch(gpu, [5, 1], [3000, 2600], 8, 2, 64, 32, "f16", seed=21)
+    for window in (300, 700, 1000, 2047, 2999, 5000):
+        case(f"attention split window {window}")
+        b.check(window=window)
+    b.free()
+
+
 @pytest.mark.parametrize("kv", ["f16", "f32"])
 @pytest.mark.parametrize("news,pasts,max_len", [([1], [5000], None), ([5, 1, 2], [3000, 1, 900], None),
                                                 ([70], [2500], None), ([1, 1], [4097, 130], 1), ([40], [2000], 0)])
@@ -253,6 +262,44 @@ def test_attention_masked_infinities(gpu, n, kv):
     assert np.all(np.isnan(last[0, :, 3])) and np.all(np.isnan(last[1]))
     d = keep[0]
     assert np.all(np.isfinite(last[0][:, d]))
+    b.free()
+
+
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("n", [1, 6, 40, 90])
+def test_attention_attended_infinities(gpu, n, kv):
+    """Infinities among the values and keys that every row attends, deep inside the context: the formula's infinity, NaN
+    where two of them cancel, nothing else touched; a key of -inf for positive queries has no weight."""
+    case(f"attention attended infinities, chunk of {n}, {kv}")
+
+    def spoil(b):
+        b.V[0][100, 0, 3] = np.inf
+        b.V[0][101, 0, 4] = -np.inf
+        b.V[0][102, 0, 5], b.V[0][103, 0, 5] = np.inf, -np.inf
+        b.V[0][104, 1, 6] = np.nan
+        b.K[0][200] = -np.inf
+        b.V[0][200] = 1000.0
+    b = Batch(gpu, [n], [300], 8, 2, 64, 16, kv, seed=n, vals=spoil)
+    b.q[:] = np.abs(b.q) + 0.25
+    b.q[:, 1] = 0.5                                    # exact in few bits: the second term has nothing left
+    b.dq.upload(b.q)
+    got = b.attend().reshape(n, 2, 4, 64)
+    assert np.all(got[:, 0, :, 3] == np.inf) and np.all(got[:, 0, :, 4] == -np.inf)
+    assert np.all(np.isnan(got[:, 0, :, 5])) and np.all(np.isnan(got[:, 1, :, 6]))
+    for i, d in ((100, 3), (101, 4), (102, 5), (103, 5)):
+        b.V[0][i, 0, d] = 0
+    b.V[0][104, 1, 6] = 0
+    with np.errstate(all="ignore"):
+        b.K[0][200] = -60000.0                         # no weight either
+        exp, _ = b.expect()
+        b.K[0][200] = 0
+        _, tol = b.expect()
+    exp, tol = exp.reshape(n, 2, 4, 64), tol.reshape(n, 2, 4, 64)
+    keep = np.ones((2, 64), bool)
+    keep[0, 3:6] = keep[1, 6] = False
+    for h in range(2):
+        d = keep[h]
+        assert np.all(np.abs(got - exp)[:, h][..., d] <= tol[:, h][..., d])
     b.free()
 
 
