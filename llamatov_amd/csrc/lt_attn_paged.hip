@@ -126,43 +126,113 @@ __device__ __forceinline__ float sum_over_groups(float a) {
 // accumulator is tied to a wait in the block that computed it.
 template <int D, int N>
 __device__ __forceinline__ void settle_all(f32x4 (&o)[D][N]) {
-  static_assert(D % 4 == 0 && (N == 1 || N == 2), "settle_all: accumulators");
+  static_assert(N == 1 || N == 2, "settle_all: accumulators");
 #pragma unroll
-  for (int d = 0; d < D; d += 4) {
-    if constexpr (N == 1)
-      asm volatile("s_nop 15" : "+v"(o[d][0]), "+v"(o[d + 1][0]), "+v"(o[d + 2][0]), "+v"(o[d + 3][0]));
-    else
-      asm volatile("s_nop 15"
-                   : "+v"(o[d][0]), "+v"(o[d][1]), "+v"(o[d + 1][0]), "+v"(o[d + 1][1]), "+v"(o[d + 2][0]),
-                     "+v"(o[d + 2][1]), "+v"(o[d + 3][0]), "+v"(o[d + 3][1]));
+  for (int d = 0; d + 2 <= D; d += 2) {
+    if constexpr (N == 1) asm volatile("" : "+v"(o[d][0]), "+v"(o[d + 1][0]));
+    else asm volatile("" : "+v"(o[d][0]), "+v"(o[d][1]), "+v"(o[d + 1][0]), "+v"(o[d + 1][1]));
   }
+  if constexpr (N == 1) asm volatile("s_nop 15" : "+v"(o[D - 1][0]));
+  else asm volatile("s_nop 15" : "+v"(o[D - 1][0]), "+v"(o[D - 1][1]));
+}
+
+// a less its binary16 rounding in the low (high) half of h, exactly.
+__device__ __forceinline__ float rest_lo(uint32_t h, float a) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(a));
+  return r;
+}
+__device__ __forceinline__ float rest_hi(uint32_t h, float a) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(a));
+  return r;
 }
 
 // Two fp32 values as two binary16 terms each.
 __device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
-  const f16x2 h = __builtin_convertvector((f32x2){a, b}, f16x2);
-  *hi = __builtin_bit_cast(uint32_t, h);
-  *lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a - (float)h.x, b - (float)h.y}, f16x2));
+  const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
+  *hi = h;
+  *lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){rest_lo(h, a), rest_hi(h, b)}, f16x2));
 }
 
-// The same for a query, whose terms also multiply keys of infinity: both terms have q's sign and are zero only
-// where q is, so that their products with one add up to what q's own is (the least binary16 in place of a zero: 2^-38
-// of the row's largest).
-__device__ __forceinline__ uint16_t same_sign(float x, float q) {
-  const uint16_t h = __builtin_bit_cast(uint16_t, (_Float16)x);
-  return (h & 0x7FFFu) == 0 && q != 0.0f ? (uint16_t)((__float_as_uint(q) >> 16 & 0x8000u) | 1u) : h;
-}
-__device__ __forceinline__ void split2_q(float a, float b, uint32_t* hi, uint32_t* lo) {
-  const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(a, b));   // toward zero: the rest keeps the sign
-  *hi = same_sign((float)h.x, a) | (uint32_t)same_sign((float)h.y, b) << 16;
-  *lo = same_sign(a - (float)h.x, a) | (uint32_t)same_sign(b - (float)h.y, b) << 16;
+// Elements d .. d + 3 of packed row `row` of KV head h: the result, or the split's part of it.
+__device__ __forceinline__ void put_row(const AttnArgs& A, const Tile& X, int q0, int h, int sp, int row, int d, f32x4 o,
+                                        float m, float z) {
+  const int t = row / A.rep, head = h * A.rep + row % A.rep, hd = A.C.hd;
+  const size_t r = (size_t)(q0 + t) * A.nh + head;
+  if (X.nact == 1) {
+    const bool any = key_hi(X.past, X.cap, t) > key_lo(A, X.past, t);
+    const float inv = 1.0f / z;
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] = any ? o[e] * inv : 0.0f;
+    float* to = A.out + r * hd + d;
+    if (A.vec) {
+      *(f32x4*)to = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) to[e] = o[e];
+    }
+  } else {
+    const size_t at = r * A.nsplit + sp;
+    *(f32x4*)(A.ws.o + at * hd + d) = o;
+    if (d == 0) {
+      A.ws.m[at] = m;
+      A.ws.z[at] = z;
+    }
+  }
 }
 
-// The binary16 halves of w that are not finite become zero; true when there were any.
-__device__ __forceinline__ bool drop_nonfinite(uint32_t* w) {
-  const bool l = (*w & 0x7C00u) == 0x7C00u, h = (*w & 0x7C000000u) == 0x7C000000u;
-  *w &= (l ? 0xFFFF0000u : 0xFFFFFFFFu) & (h ? 0x0000FFFFu : 0xFFFFFFFFu);
-  return l || h;
+// A tile's rows over keys k0 .. k1 - 1 by the formula itself, a wave a row: lane j scores key j of each 64, then sums
+// the values' dimensions 4 j ..  Taken where the matrix products met what is not finite: a masked value of infinity times a
+// weight of zero, or an infinity times two terms of different signs, is NaN there and nothing or an infinity here.
+template <int TM, int WAVES, bool F16>
+__device__ __forceinline__ void rows_one_by_one(const AttnArgs& A, const Tile& X, int b, int h, int k0, int k1, int sp) {
+  const PagedKv& C = A.C;
+  const int lane = threadIdx.x & 63, hd = C.hd, q0 = A.q_start[b];
+  auto at = [](const void* c, size_t i) { return F16 ? lt_h2f(((const uint16_t*)c)[i]) : ((const float*)c)[i]; };
+  for (int i = threadIdx.x >> 6; i < TM && X.row0 + i < X.rows; i += WAVES) {
+    const int row = X.row0 + i, t = row / A.rep;
+    const float* q = A.q + (size_t)(q0 + t) * A.q_stride + (size_t)(h * A.rep + row % A.rep) * hd;
+    int lo = key_lo(A, X.past, t), end = key_hi(X.past, X.cap, t);
+    lo = lo < k0 ? k0 : lo;
+    end = end > k1 ? k1 : end;
+    float m = -__builtin_inff(), z = 0.0f;
+    f32x4 o = {0, 0, 0, 0};
+    for (int k = lo; k < end && !(z != z); k += 64) {   // a row with a NaN among its weights is NaN
+      const int key = k + lane;
+      const int pg = key < end ? page_of(C, b, key) : -1;
+      float s = -__builtin_inff();
+      if (key < end) {
+        s = 0.0f;
+        const size_t kr = pg >= 0 ? paged_row(C, pg, h, key) : 0;
+#pragma unroll 1
+        for (int d = 0; pg >= 0 && d < hd; d++) s = fmaf(q[d], at(C.kc, kr + d), s);
+        s = s * (A.scale * A.sign * kLog2e);
+      }
+      float mt = s;
+#pragma unroll
+      for (int x = 32; x; x >>= 1) mt = fmaxf(mt, __shfl_xor(mt, x, 64));
+      const float mn = fmaxf(m, mt), mu = mn == -__builtin_inff() ? 0.0f : mn;
+      const float a = __builtin_amdgcn_exp2f(m - mu), p = __builtin_amdgcn_exp2f(s - mu + kPShift);
+      float zt = p;
+#pragma unroll
+      for (int x = 32; x; x >>= 1) zt += __shfl_xor(zt, x, 64);
+      z = fmaf(z, a, zt);
+      m = mn;
+      o *= a;
+#pragma unroll 1
+      for (int j = 0; j < 64 && k + j < end; j++) {
+        const int pj = __shfl(pg, j, 64);
+        const float w = __shfl(p, j, 64);
+        if (pj < 0 || lane * 4 >= hd) continue;
+        const size_t vr = paged_row(C, pj, h, k + j) + lane * 4;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = fmaf(w, at(C.vc, vr + e), o[e]);
+      }
+    }
+    if (z != z) o = (f32x4){z, z, z, z};
+    if (lane * 4 < hd) put_row(A, X, q0, h, sp, row, lane * 4, o, m, z);
+  }
 }
 
 // HDP: head dim rounded up to 64, 128 or 256.  A wave takes NT tiles of 16 rows; RW waves take different rows and
@@ -189,7 +259,7 @@ template <int HDP, int NT, int RW, int KW, int KT, bool F16, int WPE>
 __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
   using G = Cfg<HDP, NT, RW, KW, KT, F16>;
   constexpr int CPR = G::kCpr, MT = KT / 16, DT = HDP / 16, KC = F16 ? HDP / 32 : HDP / 16;
-  extern __shared__ __attribute__((aligned(256))) uint8_t smem[];
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];   // a row's chunks change by xor
   const PagedKv& C = A.C;
   const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -252,7 +322,7 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
 #pragma unroll
         for (int j = 0; j < W; j += 2) {
           uint32_t a, e;
-          split2_q(v[c][j] * up, v[c][j + 1] * up, &a, &e);
+          split2(v[c][j] * up, v[c][j + 1] * up, &a, &e);
           qh[nt][c][j / 2] = a;
           ql[nt][c][j / 2] = e;
         }
@@ -264,6 +334,8 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
         for (int j = 0; j < W; j++) qh[nt][c][j] = __float_as_uint(v[c][j] * A.sign);
     }
   }
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) f[nt] = fmaxf(f[nt], 0x1.0p-126f);   // a scale of zero: scores of -inf stay that
   // the wave's rows as a whole
   const int wrows = rw0 + 16 * NT < X.rows ? 16 * NT : X.rows - rw0;
   const int tw0 = rw0 / A.rep, tw1 = (rw0 + wrows - 1) / A.rep;
@@ -273,27 +345,37 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
   // ---- key tiles into LDS -------------------------------------------------------------------------
   const uint32_t ring = (uint32_t)(uintptr_t)(lds_u8*)smem + kw * 2 * G::kStageB;
   const size_t row_b = (size_t)C.hd * (F16 ? 2 : 4);
-  // byte offset of the pool row of key k + lane (lanes below KT), or -1: no row, or a page outside the pool
-  auto look_up = [&](int k) -> long long {
+  const ptrdiff_t v_off = (ptrdiff_t)((uintptr_t)C.vc - (uintptr_t)C.kc);
+  // the K pool's row of key k + lane (lanes below KT), or null: no key of this tile, or a page outside the pool
+  auto look_up = [&](int k) -> const uint8_t* {
     const int key = k + lane;
-    if (lane >= KT || key < X.lo || key >= k1) return -1;
+    if (lane >= KT || key < X.lo || key >= k1) return nullptr;
     const int pg = page_of(C, b, key);
     if (pg < 0) {
       if (A.err) *A.err = 1;
-      return -1;
+      return nullptr;
     }
-    return (long long)((((size_t)pg * C.nkv + h) << C.shift) + (key & ((1 << C.shift) - 1))) * row_b;
+    return (const uint8_t*)C.kc + ((((size_t)pg * C.nkv + h) << C.shift) + (key & ((1 << C.shift) - 1))) * row_b;
   };
-  auto stage = [&](long long off, int buf) {
+  auto stage = [&](const uint8_t* rows, int buf) {
+    int ln = lane;
+    asm volatile("" : "+v"(ln));   // what follows from the lane is formed here, not kept over the loop
+    const bool whole = __all(rows != nullptr || lane >= KT) && row_b == G::kRowB;
 #pragma unroll
     for (int i = 0; i < G::kLoads; i++) {
-      const int first = (i * RW + rw) * 64, slot = first + lane;
-      const int row = slot / CPR, c = (slot % CPR) ^ swz<CPR>(row);
-      const long long o = __shfl(off, row, 64);
-      const bool on = o >= 0 && (size_t)c * 16 < row_b;
-      const uint8_t* kp = on ? (const uint8_t*)C.kc + o + c * 16 : (const uint8_t*)&g_zero16;
-      const uint8_t* vp = on ? (const uint8_t*)C.vc + o + c * 16 : (const uint8_t*)&g_zero16;
+      const int first = (i * RW + rw) * 64;
+      const int row = first / CPR + ln / CPR, c = (ln % CPR) ^ swz<CPR>(row);
+      const uint8_t* kp = (const uint8_t*)__shfl((long long)rows, row, 64);
       const uint32_t to = ring + buf * G::kStageB + first * 16;
+      const uint8_t* vp;
+      if (whole) {
+        kp += c * 16;
+        vp = kp + v_off;
+      } else {
+        const bool on = kp != nullptr && c * 16 < (int)row_b;
+        vp = on ? kp + v_off + c * 16 : (const uint8_t*)&g_zero16;
+        kp = on ? kp + c * 16 : (const uint8_t*)&g_zero16;
+      }
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(kp) : "memory", "m0");
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to + G::kTileB), "v"(vp)
                    : "memory", "m0");
@@ -303,14 +385,16 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
   // ---- one key tile -------------------------------------------------------------------------------
   f32x4 acc[DT][NT];
   float mref[NT], z[NT];
-  const uint32_t ka0 = n16 * G::kRowB + ((g ^ swz<CPR>(n16)) << 4);             // step c: ^ (c << 6)
+  const uint32_t ka0 = ring + n16 * G::kRowB + ((g ^ swz<CPR>(n16)) << 4);                        // step c: ^ (c << 6)
   const int vr = 4 * g + (n16 >> 2);
-  const uint32_t va0 = vr * G::kRowB + ((((n16 >> 1) & 1) ^ swz<CPR>(vr)) << 4) + (n16 & 1) * 8;   // fp16: ^ (d << 5)
+  const uint32_t va0 = ring + G::kTileB +
+                       (F16 ? vr * G::kRowB + ((((n16 >> 1) & 1) ^ swz<CPR>(vr)) << 4) + (n16 & 1) * 8   // dim tile d: ^ (d << 5)
+                            : 4 * g * G::kRowB + (n16 & 3) * 4);
   auto lds = [](uint32_t a) { return (lds_u8*)(uintptr_t)a; };
 
-  auto compute = [&](int k, int buf, auto masked) {
-    constexpr bool M = decltype(masked)::value;
-    const uint32_t kb = ring + buf * G::kStageB, vb = kb + G::kTileB;
+  auto compute = [&](int k, int buf, bool masked) {
+    uint32_t ka = ka0 + buf * G::kStageB, va = va0 + buf * G::kStageB;
+    asm volatile("" : "+v"(ka), "+v"(va));   // the addresses of the steps are formed here, not kept over the loop
     f32x4 s[MT][NT];
 #pragma unroll
     for (int m = 0; m < MT; m++)
@@ -320,7 +404,7 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
     for (int c = 0; c < KC; c++)
 #pragma unroll
       for (int m = 0; m < MT; m++) {
-        const u32x4 a = *(const __attribute__((address_space(3))) u32x4*)lds(kb + m * 16 * G::kRowB + (ka0 ^ (c << 6)));
+        const u32x4 a = *(const __attribute__((address_space(3))) u32x4*)lds((ka ^ (c << 6)) + m * 16 * G::kRowB);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
           if constexpr (F16) {
@@ -334,7 +418,20 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
           }
         }
       }
-    // scores in base-2 units, their maxima, the reference
+    settle_all(s);
+    if (masked) {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+        const int first = k + 4 * g - lo[nt];
+        const uint32_t width = hi[nt] - lo[nt];
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            s[m][nt][i] = (uint32_t)(first + 16 * m + i) < width ? s[m][nt][i] : -__builtin_inff();
+      }
+    }
+    // this lane's largest scores; the reference moves only when one passes it by kSlack
     float mt[NT];
     bool moved = false;
 #pragma unroll
@@ -343,22 +440,14 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
 #pragma unroll
       for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          float x = s[m][nt][i] * f[nt];
-          if constexpr (M) {
-            const int key = k + 16 * m + 4 * g + i;
-            x = key < hi[nt] && key >= lo[nt] ? x : -__builtin_inff();
-          }
-          s[m][nt][i] = x;
-          mt[nt] = fmaxf(mt[nt], x);
-        }
-      mt[nt] = max_over_groups(mt[nt]);
+        for (int i = 0; i < 4; i++) mt[nt] = fmaxf(mt[nt], s[m][nt][i]);
+      mt[nt] *= f[nt];
       moved |= mt[nt] > mref[nt] + kSlack;
     }
     if (__any(moved)) {
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
-        const float mn = fmaxf(mref[nt], mt[nt]);
+        const float mn = fmaxf(mref[nt], max_over_groups(mt[nt]));
         const float al = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(mref[nt] - mn);
         mref[nt] = mn;
         z[nt] *= al;
@@ -373,11 +462,10 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
       for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          s[m][nt][i] = __builtin_amdgcn_exp2f(s[m][nt][i] + bias);
+          s[m][nt][i] = __builtin_amdgcn_exp2f(fmaf(s[m][nt][i], f[nt], bias));
           z[nt] += s[m][nt][i];
         }
     }
-    bool bad = false;   // a masked tile's V values that are not finite are left to put_nonfinite
     if constexpr (F16) {
       u32x4 ph[MT / 2][NT], pl[MT / 2][NT];
 #pragma unroll
@@ -395,17 +483,12 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
       for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int kk = 0; kk < MT / 2; kk++) {
-          const uint32_t at = vb + kk * 32 * G::kRowB + (va0 ^ (d << 5));
+          const uint32_t at = (va ^ (d << 5)) + kk * 32 * G::kRowB;
           typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
           const i16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)lds(at));
           const i16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)lds(at + 16 * G::kRowB));
           const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
-          uint32_t w[4] = {w0.x, w0.y, w1.x, w1.y};
-          if constexpr (M) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) bad |= drop_nonfinite(&w[j]);
-          }
-          const f16x8 av = __builtin_bit_cast(f16x8, (u32x4){w[0], w[1], w[2], w[3]});
+          const f16x8 av = __builtin_bit_cast(f16x8, (u32x4){w0.x, w0.y, w1.x, w1.y});
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) {
             acc[d][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, __builtin_bit_cast(f16x8, ph[kk][nt]), acc[d][nt], 0, 0, 0);
@@ -414,138 +497,66 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
         }
     } else {
 #pragma unroll
-      for (int m = 0; m < MT; m++)
+      for (int i = 0; i < 4; i++) {
+        const int sw = swz<CPR>(4 * g + i);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int r = 4 * g + i;
-          const uint32_t rb = vb + (m * 16 + r) * G::kRowB + (n16 & 3) * 4;
+        for (int d = 0; d < DT; d++) {
+          const uint32_t at = va + (((4 * d + (n16 >> 2)) ^ sw) << 4) + i * G::kRowB;
 #pragma unroll
-          for (int d = 0; d < DT; d++) {
-            const uint32_t at = rb + (((4 * d + (n16 >> 2)) ^ swz<CPR>(r)) << 4);
-            uint32_t w = *(const __attribute__((address_space(3))) uint32_t*)lds(at);
-            if constexpr (M) {
-              if ((w & 0x7F800000u) == 0x7F800000u) {
-                w = 0;
-                bad = true;
-              }
-            }
+          for (int m = 0; m < MT; m++) {
+            const float w = *(const __attribute__((address_space(3))) float*)lds(at + m * 16 * G::kRowB);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) acc[d][nt] = mma(__uint_as_float(w), s[m][nt][i], acc[d][nt]);
+            for (int nt = 0; nt < NT; nt++) acc[d][nt] = mma(w, s[m][nt][i], acc[d][nt]);
           }
         }
-    }
-    settle_all(acc);
-    if constexpr (M) {
-      if (__any(bad)) {
-        // the values that are not finite, key by key, for the rows that attend the key
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-#pragma unroll 1
-            for (int gg = 0; gg < 4; gg++) {
-              const int r = 4 * gg + i, key = k + 16 * m + r;
-              float p[NT];
-              bool on[NT];
-#pragma unroll
-              for (int nt = 0; nt < NT; nt++) {
-                p[nt] = __shfl(s[m][nt][i], gg * 16 + n16, 64);
-                on[nt] = key < hi[nt] && key >= lo[nt];
-              }
-              const uint32_t rb = vb + (m * 16 + r) * G::kRowB;
-#pragma unroll
-              for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                  float v;
-                  if constexpr (F16) {
-                    const int c = 2 * d + (g >> 1);
-                    v = lt_h2f(*(const __attribute__((address_space(3))) uint16_t*)lds(
-                        rb + ((c ^ swz<CPR>(r)) << 4) + (g & 1) * 8 + e * 2));
-                  } else {
-                    v = *(const __attribute__((address_space(3))) float*)lds(rb + (((4 * d + g) ^ swz<CPR>(r)) << 4) + e * 4);
-                  }
-                  if (!__builtin_isfinite(v)) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-                      if (on[nt]) acc[d][nt][e] = fmaf(p[nt], v, acc[d][nt][e]);
-                  }
-                }
-            }
       }
     }
+    settle_all(acc);
   };
 
   // ---- the split's tiles: while one is computed, the next is on its way ----------------------------
   const int ntiles = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0, iters = (ntiles + KW - 1) / KW;
   auto tile_key = [&](int it) { return k0 + (it * KW + kw) * KT; };
-  // A value of infinity that is attended meets a weight's two terms one by one, and the second may be zero or
-  // negative: a NaN in the result sends the workgroup over its tiles again with such values taken apart everywhere.
-  bool careful = false;
-  for (;;) {
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      mref[nt] = -__builtin_inff();
-      z[nt] = 0.0f;
+  for (int nt = 0; nt < NT; nt++) {
+    mref[nt] = -__builtin_inff();
+    z[nt] = 0.0f;
 #pragma unroll
-      for (int d = 0; d < DT; d++) acc[d][nt] = (f32x4){0, 0, 0, 0};
-    }
-    if (iters > 0) {
-      stage(look_up(tile_key(0)), 0);
-      long long off = look_up(tile_key(1));
-      for (int it = 0; it < iters; it++) {
-        // this tile has come, and what was read of the one before it has left the buffer that is filled next
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        if constexpr (RW > 1) __syncthreads();
-        if (it + 1 < iters) {
-          stage(off, (it + 1) & 1);
-          off = look_up(tile_key(it + 2));
-        }
-        const int k = tile_key(it);
-        if (k < k1 && k < whi1 && k + KT > wlo0) {
-          if (careful || k < wlo1 || k + KT > whi0) compute(k, it & 1, std::true_type{});
-          else compute(k, it & 1, std::false_type{});
-        }
+    for (int d = 0; d < DT; d++) acc[d][nt] = (f32x4){0, 0, 0, 0};
+  }
+  if (iters > 0) {
+    stage(look_up(tile_key(0)), 0);
+    const uint8_t* next = look_up(tile_key(1));
+    for (int it = 0; it < iters; it++) {
+      // this tile has come, and what was read of the one before it has left the buffer that is filled next
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      if constexpr (RW > 1) __syncthreads();
+      if (it + 1 < iters) {
+        stage(next, (it + 1) & 1);
+        next = look_up(tile_key(it + 2));
       }
+      const int k = tile_key(it);
+      if (k < k1 && k < whi1 && k + KT > wlo0) compute(k, it & 1, k < wlo1 || k + KT > whi0);
     }
-    if (careful) break;
-    float sum = 0.0f;   // NaN where any of them is, or where infinities of both signs meet
+  }
+  // What is not finite and was wrongly met -- a value of infinity times the zero weight of a masked key, an infinity
+  // times two terms of different signs -- is a NaN in the results; the sum is one also where infinities of both signs meet.
+  float sum = 0.0f;
 #pragma unroll
-    for (int d = 0; d < DT; d++)
+  for (int d = 0; d < DT; d++)
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++)
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) sum += acc[d][nt][e];
-    if (!F16 || !__syncthreads_or(sum != sum)) break;
-    careful = true;
+      for (int e = 0; e < 4; e++) sum += acc[d][nt][e];
+  if (__syncthreads_or(sum != sum)) {
+    rows_one_by_one<G::kTM, G::kWaves, F16>(A, X, b, h, k0, k1, sp);
+    return;
   }
 
   // ---- the groups of keys joined, and the result ---------------------------------------------------
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) z[nt] = sum_over_groups(z[nt]);
-  const bool final = X.nact == 1;
-  auto put = [&](int row, int d, f32x4 o, float m, float zz) {   // d < hd, a multiple of 4
-    const int t = row / A.rep, head = h * A.rep + row % A.rep;
-    const size_t r = (size_t)(q0 + t) * A.nh + head;
-    if (final) {
-      const bool any = key_hi(X.past, X.cap, t) > key_lo(A, X.past, t);
-      const float inv = 1.0f / zz;
-#pragma unroll
-      for (int e = 0; e < 4; e++) o[e] = any ? o[e] * inv : 0.0f;
-      float* to = A.out + r * C.hd + d;
-      if (A.vec) *(f32x4*)to = o;
-      else
-#pragma unroll
-        for (int e = 0; e < 4; e++) to[e] = o[e];
-    } else {
-      const size_t at = r * A.nsplit + sp;
-      *(f32x4*)(A.ws.o + at * C.hd + d) = o;
-      if (d == 0) {
-        A.ws.m[at] = m;
-        A.ws.z[at] = zz;
-      }
-    }
-  };
+  auto put = [&](int row, int d, f32x4 o, float m, float zz) { put_row(A, X, q0, h, sp, row, d, o, m, zz); };
   if constexpr (KW == 1) {
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -633,10 +644,10 @@ struct Plan {
   int most;          // splits of any window: what the workspace is sized for
 };
 
-// Key tiles: 32 keys (fp16) or 16 (fp32) a wave or four of them, 64 where four share rows of 64.
+// Key tiles: 32 keys (fp16) or 16 (fp32) where a wave keeps its own, 64 where four share them.
 int form_kt(Form f, int hd, bool f16) {
   if (!f16) return 16;
-  return f == kRows128 && hd <= 64 ? 64 : 32;
+  return f == kRows128 && hd <= 128 ? 64 : 32;
 }
 
 Plan make_plan(int T, int B, int nh, const PagedKv& C, bool f16, int max_q, int max_len, int window) {
@@ -674,7 +685,7 @@ int launch(lt_ctx* ctx, const AttnArgs& A, const Plan& P) {
     kernel<<<grid, threads, lds, ctx->stream>>>(A);
     return lt_check_launch("k_attn_paged");
   };
-  constexpr int KT = F16 ? 32 : 16, KT2 = F16 && HDP <= 64 ? 64 : KT, KW = HDP <= 128 ? 4 : 2, NT = HDP <= 128 ? 2 : 1;
+  constexpr int KT = F16 ? 32 : 16, KT2 = F16 && HDP <= 128 ? 64 : KT, KW = HDP <= 128 ? 4 : 2, NT = HDP <= 128 ? 2 : 1;
   switch (P.form) {
     case kDecode16:
       return go(k_attn_paged<HDP, 1, 1, KW, KT, F16, 1>, 64 * KW, Cfg<HDP, 1, 1, KW, KT, F16>::kLds);
