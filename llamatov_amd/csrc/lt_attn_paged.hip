@@ -274,6 +274,85 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
   const int k1 = sp == X.nact - 1 ? X.hi : k0 + A.chunk;
   if (X.past + (X.rows - 1) / A.rep >= X.cap && A.err && threadIdx.x == 0) *A.err = 1;
 
+  // ---- key tiles into LDS -------------------------------------------------------------------------
+  // A direct load takes 64 chunks of 16 bytes: kRpi rows of the tile, from one page unless pages are smaller than that.
+  constexpr int kRpi = 64 / CPR;
+  const uint32_t ring = (uint32_t)(uintptr_t)(lds_u8*)smem + kw * 2 * G::kStageB;
+  const uint32_t row_b = C.hd * (F16 ? 2 : 4);
+  const ptrdiff_t v_off = (ptrdiff_t)((uintptr_t)C.vc - (uintptr_t)C.kc);
+  typedef const __attribute__((address_space(4))) int const_int;
+  const_int* table = (const_int*)(uintptr_t)(C.table + (size_t)b * C.stride);
+  const int slots = (1 << C.shift) - 1;
+  // the pages of a tile's loads, read on the scalar side a tile ahead
+  struct Pages {
+    int id[G::kLoads];
+  };
+  auto look_up = [&](int k) {
+    Pages P;
+#pragma unroll
+    for (int i = 0; i < G::kLoads; i++) {
+      const int key = k + (i * RW + rw) * kRpi;
+      P.id[i] = table[(key < k1 ? key : k1 - 1) >> C.shift];
+    }
+    return P;
+  };
+  auto load16 = [](uint32_t to, const uint8_t* base, uint32_t off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base)
+                 : "memory", "m0");
+  };
+  auto load16_far = [](uint32_t to, const uint8_t* from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory", "m0");
+  };
+  auto stage = [&](int k, const Pages& P, int buf) {
+    int ln = lane;
+    asm volatile("" : "+v"(ln));   // what follows from the lane is formed here, not kept over the loop
+    const uint32_t to = ring + buf * G::kStageB + rw * 1024;
+    bool fast = k >= X.lo && k + KT <= k1 && row_b == G::kRowB && slots + 1 >= kRpi;
+#pragma unroll
+    for (int i = 0; i < G::kLoads; i++) fast = fast && (uint32_t)P.id[i] < (uint32_t)C.n_pages;
+    if (fast) {
+#pragma unroll
+      for (int i = 0; i < G::kLoads; i++) {
+        const int r0 = (i * RW + rw) * kRpi;
+        const uint8_t* kb = (const uint8_t*)C.kc +
+                            ((((size_t)P.id[i] * C.nkv + h) << C.shift) + ((k + r0) & slots)) * G::kRowB;
+        const uint32_t off = (ln / CPR) * G::kRowB + (((ln % CPR) ^ swz<CPR>(r0 + ln / CPR)) << 4);
+        load16(to + i * RW * 1024, kb, off);
+        load16(to + i * RW * 1024 + G::kTileB, kb + v_off, off);
+      }
+      return;
+    }
+    // rows past either end of the keys take the nearest one's (their weights are zero), chunks past hd and rows
+    // without a page zeros
+#pragma unroll
+    for (int i = 0; i < G::kLoads; i++) {
+      const int row = (i * RW + rw) * kRpi + ln / CPR, c = (ln % CPR) ^ swz<CPR>(row);
+      int key = k + row;
+      key = key >= k1 ? k1 - 1 : key;
+      key = key < X.lo ? X.lo : key;
+      const int pg = page_of(C, b, key);
+      if (pg < 0 && A.err) *A.err = 1;
+      const bool on = pg >= 0 && c * 16 < (int)row_b;
+      const uint8_t* kp = (const uint8_t*)C.kc + ((((size_t)(on ? pg : 0) * C.nkv + h) << C.shift) + (key & slots)) * row_b + c * 16;
+      load16_far(to + i * RW * 1024, on ? kp : (const uint8_t*)&g_zero16);
+      load16_far(to + i * RW * 1024 + G::kTileB, on ? kp + v_off : (const uint8_t*)&g_zero16);
+    }
+  };
+  const int ntiles = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0, iters = (ntiles + KW - 1) / KW;
+  auto tile_key = [&](int it) { return k0 + (it * KW + kw) * KT; };
+  // A wave that keeps its own tiles has two on their way; waves that share theirs meet once a tile and have one.
+  constexpr bool kOwn = RW == 1;
+  Pages next = {};
+  if (iters > 0) {
+    next = look_up(tile_key(0));
+    stage(tile_key(0), next, 0);
+    next = look_up(tile_key(1));
+    if (kOwn && iters > 1) {
+      stage(tile_key(1), next, 1);
+      next = look_up(tile_key(2));
+    }
+  }
+
   // this lane's rows
   const int rw0 = X.row0 + rw * 16 * NT;
   const int q0 = A.q_start[b];
@@ -341,46 +420,6 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
   const int tw0 = rw0 / A.rep, tw1 = (rw0 + wrows - 1) / A.rep;
   const int whi0 = key_hi(X.past, X.cap, tw0), whi1 = wrows > 0 ? key_hi(X.past, X.cap, tw1) : 0;
   const int wlo0 = key_lo(A, X.past, tw0), wlo1 = key_lo(A, X.past, tw1);
-
-  // ---- key tiles into LDS -------------------------------------------------------------------------
-  const uint32_t ring = (uint32_t)(uintptr_t)(lds_u8*)smem + kw * 2 * G::kStageB;
-  const size_t row_b = (size_t)C.hd * (F16 ? 2 : 4);
-  const ptrdiff_t v_off = (ptrdiff_t)((uintptr_t)C.vc - (uintptr_t)C.kc);
-  // the K pool's row of key k + lane (lanes below KT), or null: no key of this tile, or a page outside the pool
-  auto look_up = [&](int k) -> const uint8_t* {
-    const int key = k + lane;
-    if (lane >= KT || key < X.lo || key >= k1) return nullptr;
-    const int pg = page_of(C, b, key);
-    if (pg < 0) {
-      if (A.err) *A.err = 1;
-      return nullptr;
-    }
-    return (const uint8_t*)C.kc + ((((size_t)pg * C.nkv + h) << C.shift) + (key & ((1 << C.shift) - 1))) * row_b;
-  };
-  auto stage = [&](const uint8_t* rows, int buf) {
-    int ln = lane;
-    asm volatile("" : "+v"(ln));   // what follows from the lane is formed here, not kept over the loop
-    const bool whole = __all(rows != nullptr || lane >= KT) && row_b == G::kRowB;
-#pragma unroll
-    for (int i = 0; i < G::kLoads; i++) {
-      const int first = (i * RW + rw) * 64;
-      const int row = first / CPR + ln / CPR, c = (ln % CPR) ^ swz<CPR>(row);
-      const uint8_t* kp = (const uint8_t*)__shfl((long long)rows, row, 64);
-      const uint32_t to = ring + buf * G::kStageB + first * 16;
-      const uint8_t* vp;
-      if (whole) {
-        kp += c * 16;
-        vp = kp + v_off;
-      } else {
-        const bool on = kp != nullptr && c * 16 < (int)row_b;
-        vp = on ? kp + v_off + c * 16 : (const uint8_t*)&g_zero16;
-        kp = on ? kp + c * 16 : (const uint8_t*)&g_zero16;
-      }
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(kp) : "memory", "m0");
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to + G::kTileB), "v"(vp)
-                   : "memory", "m0");
-    }
-  };
 
   // ---- one key tile -------------------------------------------------------------------------------
   f32x4 acc[DT][NT];
@@ -514,9 +553,7 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
     settle_all(acc);
   };
 
-  // ---- the split's tiles: while one is computed, the next is on its way ----------------------------
-  const int ntiles = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0, iters = (ntiles + KW - 1) / KW;
-  auto tile_key = [&](int it) { return k0 + (it * KW + kw) * KT; };
+  // ---- the split's tiles ---------------------------------------------------------------------------
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
     mref[nt] = -__builtin_inff();
@@ -524,19 +561,28 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
 #pragma unroll
     for (int d = 0; d < DT; d++) acc[d][nt] = (f32x4){0, 0, 0, 0};
   }
-  if (iters > 0) {
-    stage(look_up(tile_key(0)), 0);
-    const uint8_t* next = look_up(tile_key(1));
-    for (int it = 0; it < iters; it++) {
+  for (int it = 0; it < iters; it++) {
+    const int k = tile_key(it);
+    const bool on = k < k1 && k < whi1 && k + KT > wlo0, masked = k < wlo1 || k + KT > whi0;
+    if constexpr (kOwn) {
+      // all but the loads of the tile after this one have come
+      if (it + 1 < iters) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * G::kLoads) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (on) compute(k, it & 1, masked);
+      if (it + 2 < iters) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // what was read of this buffer has left it
+        stage(tile_key(it + 2), next, it & 1);
+        next = look_up(tile_key(it + 3));
+      }
+    } else {
       // this tile has come, and what was read of the one before it has left the buffer that is filled next
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      if constexpr (RW > 1) __syncthreads();
+      __syncthreads();
       if (it + 1 < iters) {
-        stage(next, (it + 1) & 1);
+        stage(tile_key(it + 1), next, (it + 1) & 1);
         next = look_up(tile_key(it + 2));
       }
-      const int k = tile_key(it);
-      if (k < k1 && k < whi1 && k + KT > wlo0) compute(k, it & 1, k < wlo1 || k + KT > whi0);
+      if (on) compute(k, it & 1, masked);
     }
   }
   // What is not finite and was wrongly met -- a value of infinity times the zero weight of a masked key, an infinity
