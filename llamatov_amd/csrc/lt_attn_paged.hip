@@ -650,33 +650,74 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
   }
 }
 
-// The splits of one row and head joined in ascending order; rows with one split are in `out` already.
-__global__ __launch_bounds__(64) void k_attn_paged_join(AttnArgs A, int tm, int kt) {
-  const int r = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, hd = A.C.hd;
-  const int b = seq_of_row(A.q_start, A.B, r);
-  if (b < 0) return;
-  const int t = r - A.q_start[b];
-  const Tile X = tile_of(A, b, (t * A.rep + head % A.rep) / tm, tm, kt);
-  if (X.nact == 1) return;
-  const size_t row = (size_t)r * A.nh + head, at = row * A.nsplit;
-  float m = -__builtin_inff();
-  for (int s = lane; s < X.nact; s += 64) m = fmaxf(m, A.ws.m[at + s]);
-  for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
-  const bool any = key_hi(X.past, X.cap, t) > key_lo(A, X.past, t);
-  for (int d = lane * 4; d < hd; d += 256) {
-    float z = 0.0f;
-    f32x4 o = {0, 0, 0, 0};
-    for (int s = 0; s < X.nact; s++) {
-      const float ms = A.ws.m[at + s], a = ms == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ms - m);
-      z = fmaf(A.ws.z[at + s], a, z);
-      const f32x4 x = *(const f32x4*)(A.ws.o + (at + s) * hd + d);
-#pragma unroll
-      for (int e = 0; e < 4; e++) o[e] = fmaf(x[e], a, o[e]);
-    }
-    const float inv = 1.0f / z;
-#pragma unroll
-    for (int e = 0; e < 4; e++) A.out[row * hd + d + e] = any ? o[e] * inv : 0.0f;
+// The splits of a row and head joined; rows with one split are in `out` already.  An item (row and head) takes
+// `groups` groups of hd / 4 lanes, at least a wave: group i sums splits i, i + groups, .. in ascending order, then the
+// groups are joined in ascending order through LDS (the order depends on the sizes alone).
+__global__ __launch_bounds__(256) void k_attn_paged_join(AttnArgs A, int tm, int kt, int lanes, int groups) {
+  __shared__ __attribute__((aligned(16))) float so[256 * 4];
+  __shared__ float sm[256], sz[256];
+  const int hd = A.C.hd, per = lanes * groups;
+  const int sub = threadIdx.x / per, in = threadIdx.x % per, grp = in / lanes, d = in % lanes * 4;
+  const long long item = (long long)blockIdx.x * (256 / per) + sub;
+  const int r = __builtin_amdgcn_readfirstlane((int)(item / A.nh)), head = __builtin_amdgcn_readfirstlane((int)(item % A.nh));
+  const int b = r < A.T ? seq_of_row(A.q_start, A.B, r) : -1;
+  Tile X = {};
+  int t = 0;
+  if (b >= 0) {
+    t = r - A.q_start[b];
+    X = tile_of(A, b, (t * A.rep + head % A.rep) / tm, tm, kt);
   }
+  const bool on = b >= 0 && X.nact > 1;
+  const size_t row = (size_t)r * A.nh + head, at = row * A.nsplit;
+  float m = -__builtin_inff(), z = 0.0f;
+  f32x4 o = {0, 0, 0, 0};
+  if (on && d < hd) {
+    for (int s = grp; s < X.nact; s += 4 * groups) {
+      float ms[4], zs[4];
+      f32x4 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int sj = s + j * groups;
+        const bool in_range = sj < X.nact;
+        ms[j] = in_range ? A.ws.m[at + sj] : -__builtin_inff();
+        zs[j] = in_range ? A.ws.z[at + sj] : 0.0f;
+        x[j] = in_range ? *(const f32x4*)(A.ws.o + (at + sj) * hd + d) : (f32x4){0, 0, 0, 0};
+      }
+      const float mn = fmaxf(fmaxf(m, fmaxf(ms[0], ms[1])), fmaxf(ms[2], ms[3]));
+      const float a0 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+      z *= a0;
+      o *= a0;
+      m = mn;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float a = ms[j] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ms[j] - mn);
+        z = fmaf(zs[j], a, z);
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = fmaf(x[j][e], a, o[e]);
+      }
+    }
+  }
+  *(f32x4*)(so + threadIdx.x * 4) = o;
+  sm[threadIdx.x] = m;
+  sz[threadIdx.x] = z;
+  __syncthreads();
+  if (!on || grp != 0 || d >= hd) return;
+  float M = -__builtin_inff();
+  for (int i = 0; i < groups; i++) M = fmaxf(M, sm[threadIdx.x + i * lanes]);
+  z = 0.0f;
+  o = (f32x4){0, 0, 0, 0};
+  for (int i = 0; i < groups; i++) {
+    const int w = threadIdx.x + i * lanes;
+    const float a = sm[w] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(sm[w] - M);
+    z = fmaf(sz[w], a, z);
+    const f32x4 x = *(const f32x4*)(so + w * 4);
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] = fmaf(x[e], a, o[e]);
+  }
+  const bool any = key_hi(X.past, X.cap, t) > key_lo(A, X.past, t);
+  const float inv = 1.0f / z;
+#pragma unroll
+  for (int e = 0; e < 4; e++) A.out[row * hd + d + e] = any ? o[e] * inv : 0.0f;
 }
 
 // ---- the launch ------------------------------------------------------------------------------------
@@ -731,12 +772,12 @@ int launch(lt_ctx* ctx, const AttnArgs& A, const Plan& P) {
     kernel<<<grid, threads, lds, ctx->stream>>>(A);
     return lt_check_launch("k_attn_paged");
   };
-  constexpr int KT = F16 ? 32 : 16, KT2 = F16 && HDP <= 128 ? 64 : KT, KW = HDP <= 128 ? 4 : 2, NT = HDP <= 128 ? 2 : 1;
+  constexpr int KT = F16 ? 32 : 16, KT2 = F16 && HDP <= 128 ? 64 : KT, KW = 2, NT = HDP <= 128 ? 2 : 1;
   switch (P.form) {
     case kDecode16:
       return go(k_attn_paged<HDP, 1, 1, KW, KT, F16, 1>, 64 * KW, Cfg<HDP, 1, 1, KW, KT, F16>::kLds);
     case kDecode32:
-      if constexpr (HDP <= 128) return go(k_attn_paged<HDP, 2, 1, 4, KT, F16, 1>, 256, Cfg<HDP, 2, 1, 4, KT, F16>::kLds);
+      if constexpr (HDP <= 128) return go(k_attn_paged<HDP, 2, 1, KW, KT, F16, 1>, 64 * KW, Cfg<HDP, 2, 1, KW, KT, F16>::kLds);
       break;
     case kRows64:
       if constexpr (HDP <= 128) return go(k_attn_paged<HDP, 2, 2, 2, KT, F16, 1>, 256, Cfg<HDP, 2, 2, 2, KT, F16>::kLds);
@@ -792,7 +833,13 @@ int lt_attn_paged(lt_ctx* ctx, const float* q, int q_stride, int T, const int* q
   else if (C.hd <= 128) rc = f16 ? launch<128, true>(ctx, A, P) : launch<128, false>(ctx, A, P);
   else rc = f16 ? launch<256, true>(ctx, A, P) : launch<256, false>(ctx, A, P);
   if (rc || P.nsplit == 1) return rc;
-  k_attn_paged_join<<<dim3(T, nh), 64, 0, ctx->stream>>>(A, P.tm, P.kt);
+  // lanes for the head dim; groups for the splits, to a wave at least and a workgroup at most
+  int lanes = 1, groups = 1;
+  while (lanes * 4 < C.hd) lanes *= 2;
+  while (groups < P.nsplit && lanes * groups < 256) groups *= 2;
+  while (lanes * groups < 64) groups *= 2;
+  const long long items = (long long)T * nh, per = 256 / (lanes * groups);
+  k_attn_paged_join<<<(unsigned)((items + per - 1) / per), 256, 0, ctx->stream>>>(A, P.tm, P.kt, lanes, groups);
   return lt_check_launch("k_attn_paged_join");
 }
 
