@@ -34,6 +34,21 @@ constexpr int kMaxSplits = 128;
 
 __device__ const u32x4 g_zero16 = {0, 0, 0, 0};   // what a row without a page reads
 
+// x / d for any 32-bit x by a multiplication (Granlund and Montgomery, "Division by invariant integers using
+// multiplication", PLDI 1994).
+struct Div {
+  uint32_t m, s1, s2;
+};
+inline Div make_div(uint32_t d) {
+  int l = 0;
+  while ((1ull << l) < d) l++;
+  return {(uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1), (uint32_t)(l < 1 ? l : 1), (uint32_t)(l < 1 ? 0 : l - 1)};
+}
+__device__ __forceinline__ int div_by(const Div& D, int x) {
+  const uint32_t hi = __umulhi((uint32_t)x, D.m);
+  return (int)((((uint32_t)x - hi) >> D.s1) + hi >> D.s2);
+}
+
 struct AttnArgs {
   const float* q;
   int q_stride;
@@ -49,10 +64,12 @@ struct AttnArgs {
   int vec;           // q rows are 16-byte aligned
   int chunk, nsplit; // keys a split, splits in the grid
   AttnWs ws;
+  Div by_rep, by_chunk, by_nkv, by_nh;
 };
 
 // One tile of a sequence's rows and the keys it attends.
 struct Tile {
+  int q0;            // the sequence's first row in the batch
   int row0, rows;    // packed rows of the sequence from row0, and its count of them
   int past, cap;
   int lo, hi;        // keys any of its rows attends
@@ -69,18 +86,25 @@ __device__ __forceinline__ int key_hi(int past, int cap, int t) {
   return p1 < cap ? p1 : cap;
 }
 
-__device__ __forceinline__ Tile tile_of(const AttnArgs& A, int b, int tile, int tm, int kt) {
+// Ints that no kernel of this file writes, for loads on the scalar side.
+typedef const __attribute__((address_space(4))) int const_int;
+__device__ __forceinline__ const_int* scalar_ints(const int* p) { return (const_int*)(uintptr_t)p; }
+
+// Rows q_start[b] .. of sequence b, none where the two do not make sense.
+__device__ __forceinline__ int rows_of(int s, int e, int T) { return s >= 0 && e > s && e <= T ? e - s : 0; }
+
+__device__ __forceinline__ Tile tile_of(const AttnArgs& A, int q0, int q1, int L, int tile, int tm, int kt) {
   Tile X;
+  X.q0 = q0;
   X.cap = A.C.stride << A.C.shift;
-  const int L = A.len[b];
   X.past = L < 0 ? 0 : L < X.cap ? L : X.cap;
   X.row0 = tile * tm;
-  X.rows = (A.q_start[b + 1] - A.q_start[b]) * A.rep;
+  X.rows = rows_of(q0, q1, A.T) * A.rep;
   const int last = X.row0 + tm < X.rows ? X.row0 + tm - 1 : X.rows - 1;
-  X.lo = key_lo(A, X.past, X.row0 / A.rep);
-  X.hi = key_hi(X.past, X.cap, last / A.rep);
+  X.lo = key_lo(A, X.past, div_by(A.by_rep, X.row0));
+  X.hi = key_hi(X.past, X.cap, div_by(A.by_rep, last));
   X.kbeg = X.lo & ~(kt - 1);
-  const int n = X.hi > X.kbeg ? (X.hi - X.kbeg + A.chunk - 1) / A.chunk : 1;
+  const int n = X.hi > X.kbeg ? div_by(A.by_chunk, X.hi - X.kbeg + A.chunk - 1) : 1;
   X.nact = n < A.nsplit ? n : A.nsplit;
   return X;
 }
@@ -92,8 +116,7 @@ __device__ __forceinline__ void find_tile(const AttnArgs& A, int x, int tm, int*
   for (int c = 0; c < A.B; c += 64) {
     int n = 0;
     if (c + lane < A.B) {
-      const int s = A.q_start[c + lane], e = A.q_start[c + lane + 1];
-      n = s >= 0 && e > s && e <= A.T ? ((e - s) * A.rep + tm - 1) / tm : 0;
+      n = (rows_of(A.q_start[c + lane], A.q_start[c + lane + 1], A.T) * A.rep + tm - 1) / tm;   // tm: a constant
     }
     int sum = n;
 #pragma unroll
@@ -156,10 +179,10 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t*
 }
 
 // Elements d .. d + 3 of packed row `row` of KV head h: the result, or the split's part of it.
-__device__ __forceinline__ void put_row(const AttnArgs& A, const Tile& X, int q0, int h, int sp, int row, int d, f32x4 o,
+__device__ __forceinline__ void put_row(const AttnArgs& A, const Tile& X, int h, int sp, int row, int d, f32x4 o,
                                         float m, float z) {
-  const int t = row / A.rep, head = h * A.rep + row % A.rep, hd = A.C.hd;
-  const size_t r = (size_t)(q0 + t) * A.nh + head;
+  const int t = div_by(A.by_rep, row), head = h * A.rep + (row - t * A.rep), hd = A.C.hd;
+  const size_t r = (size_t)(X.q0 + t) * A.nh + head;
   if (X.nact == 1) {
     const bool any = key_hi(X.past, X.cap, t) > key_lo(A, X.past, t);
     const float inv = 1.0f / z;
@@ -188,11 +211,11 @@ __device__ __forceinline__ void put_row(const AttnArgs& A, const Tile& X, int q0
 template <int TM, int WAVES, bool F16>
 __device__ __forceinline__ void rows_one_by_one(const AttnArgs& A, const Tile& X, int b, int h, int k0, int k1, int sp) {
   const PagedKv& C = A.C;
-  const int lane = threadIdx.x & 63, hd = C.hd, q0 = A.q_start[b];
+  const int lane = threadIdx.x & 63, hd = C.hd;
   auto at = [](const void* c, size_t i) { return F16 ? lt_h2f(((const uint16_t*)c)[i]) : ((const float*)c)[i]; };
   for (int i = threadIdx.x >> 6; i < TM && X.row0 + i < X.rows; i += WAVES) {
-    const int row = X.row0 + i, t = row / A.rep;
-    const float* q = A.q + (size_t)(q0 + t) * A.q_stride + (size_t)(h * A.rep + row % A.rep) * hd;
+    const int row = X.row0 + i, t = div_by(A.by_rep, row);
+    const float* q = A.q + (size_t)(X.q0 + t) * A.q_stride + (size_t)(h * A.rep + row - t * A.rep) * hd;
     int lo = key_lo(A, X.past, t), end = key_hi(X.past, X.cap, t);
     lo = lo < k0 ? k0 : lo;
     end = end > k1 ? k1 : end;
@@ -231,7 +254,7 @@ __device__ __forceinline__ void rows_one_by_one(const AttnArgs& A, const Tile& X
       }
     }
     if (z != z) o = (f32x4){z, z, z, z};
-    if (lane * 4 < hd) put_row(A, X, q0, h, sp, row, lane * 4, o, m, z);
+    if (lane * 4 < hd) put_row(A, X, h, sp, row, lane * 4, o, m, z);
   }
 }
 
@@ -255,24 +278,31 @@ __device__ __forceinline__ int swz(int r) {
   return CPR >= 16 ? (r & 15) : ((r >> 1) & 7);
 }
 
-template <int HDP, int NT, int RW, int KW, int KT, bool F16, int WPE>
-__global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
+template <bool F16>
+struct VFrag {
+  typedef u32x2 T;
+};
+template <>
+struct VFrag<false> {
+  typedef uint32_t T;
+};
+
+__device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Split sp of one tile of sequence b, KV head h; false where nothing was written because a result is not a number.
+template <int HDP, int NT, int RW, int KW, int KT, bool F16>
+__device__ __forceinline__ bool attend(const AttnArgs& A, const Tile& X, int b, int h, int sp, uint8_t* smem) {
   using G = Cfg<HDP, NT, RW, KW, KT, F16>;
   constexpr int CPR = G::kCpr, MT = KT / 16, DT = HDP / 16, KC = F16 ? HDP / 32 : HDP / 16;
-  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];   // a row's chunks change by xor
   const PagedKv& C = A.C;
   const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rw = wave % RW, kw = wave / RW;
-  const int h = blockIdx.x % C.nkv, sp = blockIdx.y;
-  int b, tile;
-  find_tile(A, blockIdx.x / C.nkv, G::kTM, &b, &tile);
-  if (b < 0) return;
-  const Tile X = tile_of(A, b, tile, G::kTM, KT);
-  if (sp >= X.nact) return;
   const int k0 = X.kbeg + sp * A.chunk;
   const int k1 = sp == X.nact - 1 ? X.hi : k0 + A.chunk;
-  if (X.past + (X.rows - 1) / A.rep >= X.cap && A.err && threadIdx.x == 0) *A.err = 1;
+  if (X.past + div_by(A.by_rep, X.rows - 1) >= X.cap && A.err && threadIdx.x == 0) *A.err = 1;
 
   // ---- key tiles into LDS -------------------------------------------------------------------------
   // A direct load takes 64 chunks of 16 bytes: kRpi rows of the tile, from one page unless pages are smaller than that.
@@ -280,8 +310,7 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
   const uint32_t ring = (uint32_t)(uintptr_t)(lds_u8*)smem + kw * 2 * G::kStageB;
   const uint32_t row_b = C.hd * (F16 ? 2 : 4);
   const ptrdiff_t v_off = (ptrdiff_t)((uintptr_t)C.vc - (uintptr_t)C.kc);
-  typedef const __attribute__((address_space(4))) int const_int;
-  const_int* table = (const_int*)(uintptr_t)(C.table + (size_t)b * C.stride);
+  const_int* table = scalar_ints(C.table + (size_t)b * C.stride);
   const int slots = (1 << C.shift) - 1;
   // the pages of a tile's loads, read on the scalar side a tile ahead
   struct Pages {
@@ -355,7 +384,6 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
 
   // this lane's rows
   const int rw0 = X.row0 + rw * 16 * NT;
-  const int q0 = A.q_start[b];
   int hi[NT], lo[NT];
   float f[NT];
   u32x4 qh[NT][KC], ql[F16 ? NT : 1][F16 ? KC : 1];
@@ -363,10 +391,10 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
   for (int nt = 0; nt < NT; nt++) {
     const int row = rw0 + nt * 16 + n16;
     const bool on = row < X.rows;
-    const int t = row / A.rep;
+    const int t = div_by(A.by_rep, row);
     hi[nt] = on ? key_hi(X.past, X.cap, t) : 0;
     lo[nt] = on ? key_lo(A, X.past, t) : 0;
-    const float* q = A.q + (size_t)(q0 + (on ? t : 0)) * A.q_stride + (size_t)(h * A.rep + (on ? row % A.rep : 0)) * C.hd;
+    const float* q = A.q + (size_t)(X.q0 + (on ? t : 0)) * A.q_stride + (size_t)(h * A.rep + (on ? row - t * A.rep : 0)) * C.hd;
     constexpr int W = F16 ? 8 : 4;   // values of a lane per step
     float v[KC][W];
 #pragma unroll
@@ -417,7 +445,7 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
   for (int nt = 0; nt < NT; nt++) f[nt] = fmaxf(f[nt], 0x1.0p-126f);   // a scale of zero: scores of -inf stay that
   // the wave's rows as a whole
   const int wrows = rw0 + 16 * NT < X.rows ? 16 * NT : X.rows - rw0;
-  const int tw0 = rw0 / A.rep, tw1 = (rw0 + wrows - 1) / A.rep;
+  const int tw0 = div_by(A.by_rep, rw0), tw1 = div_by(A.by_rep, rw0 + (wrows > 0 ? wrows : 1) - 1);
   const int whi0 = key_hi(X.past, X.cap, tw0), whi1 = wrows > 0 ? key_hi(X.past, X.cap, tw1) : 0;
   const int wlo0 = key_lo(A, X.past, tw0), wlo1 = key_lo(A, X.past, tw1);
 
@@ -430,26 +458,58 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
                        (F16 ? vr * G::kRowB + ((((n16 >> 1) & 1) ^ swz<CPR>(vr)) << 4) + (n16 & 1) * 8   // dim tile d: ^ (d << 5)
                             : 4 * g * G::kRowB + (n16 & 3) * 4);
   auto lds = [](uint32_t a) { return (lds_u8*)(uintptr_t)a; };
+  // V^T's operand of dim tile d: fp16, keys 4 g .. 4 g + 3 of key tile j of dimension n16 (a transposing read);
+  // fp32, key 4 g + j % 4 of key tile j / 4
+  auto v_frag = [&](uint32_t va, int d, int j) -> typename VFrag<F16>::T {
+    if constexpr (F16) {
+      typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+      return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)lds((va ^ (d << 5)) + j * 16 * G::kRowB)));
+    } else {
+      const int i = j & 3;
+      return *(const __attribute__((address_space(3))) uint32_t*)lds(
+          va + (((4 * d + (n16 >> 2)) ^ swz<CPR>(4 * g + i)) << 4) + i * G::kRowB + (j >> 2) * 16 * G::kRowB);
+    }
+  };
 
   auto compute = [&](int k, int buf, bool masked) {
     uint32_t ka = ka0 + buf * G::kStageB, va = va0 + buf * G::kStageB;
     asm volatile("" : "+v"(ka), "+v"(va));   // the addresses of the steps are formed here, not kept over the loop
-    f32x4 s[MT][NT];
+    auto k_frag = [&](int c, int m) {
+      return *(const __attribute__((address_space(3))) u32x4*)lds((ka ^ (c << 6)) + m * 16 * G::kRowB);
+    };
+    // A wave of its own has nothing to fill its waits with: it reads the whole tile first (its registers allow it).
+    u32x4 kf[kOwn ? KC : 1][MT];
+    typename VFrag<F16>::T vf[kOwn ? DT : 1][MT * (F16 ? 1 : 4)];
+    if constexpr (kOwn) {
+#pragma unroll
+      for (int c = 0; c < KC; c++)
+#pragma unroll
+        for (int m = 0; m < MT; m++) kf[c][m] = k_frag(c, m);
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int j = 0; j < MT * (F16 ? 1 : 4); j++) vf[d][j] = v_frag(va, d, j);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    f32x4 s[MT][NT], s2[F16 && kOwn ? MT : 1][NT];   // s2: the second term's sums, a chain of their own
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) s[m][nt] = (f32x4){0, 0, 0, 0};
+      for (int nt = 0; nt < NT; nt++) {
+        s[m][nt] = (f32x4){0, 0, 0, 0};
+        if constexpr (F16 && kOwn) s2[m][nt] = (f32x4){0, 0, 0, 0};
+      }
 #pragma unroll
     for (int c = 0; c < KC; c++)
 #pragma unroll
       for (int m = 0; m < MT; m++) {
-        const u32x4 a = *(const __attribute__((address_space(3))) u32x4*)lds((ka ^ (c << 6)) + m * 16 * G::kRowB);
+        const u32x4 a = kOwn ? kf[kOwn ? c : 0][m] : k_frag(c, m);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
           if constexpr (F16) {
-            const f16x8 ah = __builtin_bit_cast(f16x8, a);
-            s[m][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, __builtin_bit_cast(f16x8, qh[nt][c]), s[m][nt], 0, 0, 0);
-            s[m][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, __builtin_bit_cast(f16x8, ql[nt][c]), s[m][nt], 0, 0, 0);
+            f32x4& t = kOwn ? s2[kOwn ? m : 0][nt] : s[m][nt];
+            s[m][nt] = mma16(a, qh[nt][c], s[m][nt]);
+            t = mma16(a, ql[nt][c], t);
           } else {
 #pragma unroll
             for (int j = 0; j < 4; j++)
@@ -457,6 +517,12 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
           }
         }
       }
+    if constexpr (F16 && kOwn) {
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) s[m][nt] += s2[m][nt];
+    }
     settle_all(s);
     if (masked) {
 #pragma unroll
@@ -518,37 +584,45 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
             ph[m / 2][nt][(m & 1) * 2 + i / 2] = a;
             pl[m / 2][nt][(m & 1) * 2 + i / 2] = e;
           }
+      auto v_pair = [&](int d, int kk) {
+        const u32x2 w0 = kOwn ? vf[kOwn ? d : 0][2 * kk] : v_frag(va, d, 2 * kk);
+        const u32x2 w1 = kOwn ? vf[kOwn ? d : 0][2 * kk + 1] : v_frag(va, d, 2 * kk + 1);
+        return (u32x4){w0.x, w0.y, w1.x, w1.y};
+      };
+      if constexpr (kOwn) {   // an accumulator's two products far apart
 #pragma unroll
-      for (int d = 0; d < DT; d++)
+        for (int kk = 0; kk < MT / 2; kk++)
 #pragma unroll
-        for (int kk = 0; kk < MT / 2; kk++) {
-          const uint32_t at = (va ^ (d << 5)) + kk * 32 * G::kRowB;
-          typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-          const i16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)lds(at));
-          const i16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)lds(at + 16 * G::kRowB));
-          const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
-          const f16x8 av = __builtin_bit_cast(f16x8, (u32x4){w0.x, w0.y, w1.x, w1.y});
+          for (int term = 0; term < 2; term++)
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++) {
-            acc[d][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, __builtin_bit_cast(f16x8, ph[kk][nt]), acc[d][nt], 0, 0, 0);
-            acc[d][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, __builtin_bit_cast(f16x8, pl[kk][nt]), acc[d][nt], 0, 0, 0);
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+              for (int nt = 0; nt < NT; nt++)
+                acc[d][nt] = mma16(v_pair(d, kk), term ? pl[kk][nt] : ph[kk][nt], acc[d][nt]);
+      } else {
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+          for (int kk = 0; kk < MT / 2; kk++) {
+            const u32x4 av = v_pair(d, kk);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+              acc[d][nt] = mma16(av, ph[kk][nt], acc[d][nt]);
+              acc[d][nt] = mma16(av, pl[kk][nt], acc[d][nt]);
+            }
           }
-        }
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int sw = swz<CPR>(4 * g + i);
+      for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int d = 0; d < DT; d++) {
-          const uint32_t at = va + (((4 * d + (n16 >> 2)) ^ sw) << 4) + i * G::kRowB;
+        for (int d = 0; d < DT; d++)
 #pragma unroll
           for (int m = 0; m < MT; m++) {
-            const float w = *(const __attribute__((address_space(3))) float*)lds(at + m * 16 * G::kRowB);
+            const uint32_t w = kOwn ? vf[kOwn ? d : 0][m * 4 + i] : v_frag(va, d, m * 4 + i);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) acc[d][nt] = mma(w, s[m][nt][i], acc[d][nt]);
+            for (int nt = 0; nt < NT; nt++) acc[d][nt] = mma(__uint_as_float(w), s[m][nt][i], acc[d][nt]);
           }
-        }
-      }
     }
     settle_all(acc);
   };
@@ -594,15 +668,12 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
       for (int e = 0; e < 4; e++) sum += acc[d][nt][e];
-  if (__syncthreads_or(sum != sum)) {
-    rows_one_by_one<G::kTM, G::kWaves, F16>(A, X, b, h, k0, k1, sp);
-    return;
-  }
+  if (__syncthreads_or(sum != sum)) return false;
 
   // ---- the groups of keys joined, and the result ---------------------------------------------------
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) z[nt] = sum_over_groups(z[nt]);
-  auto put = [&](int row, int d, f32x4 o, float m, float zz) { put_row(A, X, q0, h, sp, row, d, o, m, zz); };
+  auto put = [&](int row, int d, f32x4 o, float m, float zz) { put_row(A, X, h, sp, row, d, o, m, zz); };
   if constexpr (KW == 1) {
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -648,6 +719,34 @@ __global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
       put(X.row0 + r, d, o, m, zz);
     }
   }
+  return true;
+}
+
+// PER_SEQ: workgroup x takes sequence x, whose rows are one tile where max_q is right (and any others one by one);
+// else tile x of the batch.
+template <int HDP, int NT, int RW, int KW, int KT, bool F16, int WPE, bool PER_SEQ>
+__global__ __launch_bounds__(64 * RW * KW, WPE) void k_attn_paged(AttnArgs A) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];   // a row's chunks change by xor
+  constexpr int TM = 16 * NT * RW;
+  const int x = div_by(A.by_nkv, blockIdx.x), h = blockIdx.x - x * A.C.nkv, sp = blockIdx.y;
+  const_int* qs = scalar_ints(A.q_start);
+  int b = x, tile = 0;
+  if constexpr (!PER_SEQ) {
+    find_tile(A, x, TM, &b, &tile);
+    if (b < 0) return;
+  }
+  const int q0 = qs[b], q1 = qs[b + 1], L = scalar_ints(A.len)[b];
+  Tile X = tile_of(A, q0, q1, L, tile, TM, KT);
+  if (X.rows == 0) return;
+  bool done = sp >= X.nact || attend<HDP, NT, RW, KW, KT, F16>(A, X, b, h, sp, smem);
+  for (;;) {
+    if (!done)
+      rows_one_by_one<TM, RW * KW, F16>(A, X, b, h, X.kbeg + sp * A.chunk,
+                                        sp == X.nact - 1 ? X.hi : X.kbeg + (sp + 1) * A.chunk, sp);
+    if (!PER_SEQ || ++tile * TM >= X.rows) break;
+    X = tile_of(A, q0, q1, L, tile, TM, KT);
+    done = sp >= X.nact;
+  }
 }
 
 // The splits of a row and head joined; rows with one split are in `out` already.  An item (row and head) takes
@@ -658,14 +757,16 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(AttnArgs A, int tm, int
   __shared__ float sm[256], sz[256];
   const int hd = A.C.hd, per = lanes * groups;
   const int sub = threadIdx.x / per, in = threadIdx.x % per, grp = in / lanes, d = in % lanes * 4;
-  const long long item = (long long)blockIdx.x * (256 / per) + sub;
-  const int r = __builtin_amdgcn_readfirstlane((int)(item / A.nh)), head = __builtin_amdgcn_readfirstlane((int)(item % A.nh));
+  const uint32_t item = blockIdx.x * (256 / per) + sub;   // T * nh < 2^31
+  const int r = __builtin_amdgcn_readfirstlane(div_by(A.by_nh, (int)item));
+  const int head = __builtin_amdgcn_readfirstlane((int)item) - r * A.nh;
   const int b = r < A.T ? seq_of_row(A.q_start, A.B, r) : -1;
   Tile X = {};
   int t = 0;
   if (b >= 0) {
-    t = r - A.q_start[b];
-    X = tile_of(A, b, (t * A.rep + head % A.rep) / tm, tm, kt);
+    const int q0 = A.q_start[b];
+    t = r - q0;
+    X = tile_of(A, q0, A.q_start[b + 1], A.len[b], (t * A.rep + (head - div_by(A.by_rep, head) * A.rep)) / tm, tm, kt);
   }
   const bool on = b >= 0 && X.nact > 1;
   const size_t row = (size_t)r * A.nh + head, at = row * A.nsplit;
@@ -726,7 +827,8 @@ enum Form { kDecode16, kDecode32, kRows64, kRows128 };
 struct Plan {
   Form form;
   int tm, kt;        // rows of a tile, keys of a key tile
-  int tiles;         // at most
+  bool per_seq;      // a workgroup a sequence: all of its rows are one tile if max_q is right
+  int tiles;         // workgroups along the batch
   int chunk, nsplit;
   int most;          // splits of any window: what the workspace is sized for
 };
@@ -748,7 +850,8 @@ Plan make_plan(int T, int B, int nh, const PagedKv& C, bool f16, int max_q, int 
   P.kt = form_kt(P.form, C.hd, f16);
   const int seqs = B < T ? B : T;
   const long long full = (long long)T * rep / P.tm;
-  P.tiles = (int)(full + seqs);
+  P.per_seq = P.form == kDecode16 || P.form == kDecode32;
+  P.tiles = P.per_seq ? B : (int)(full + seqs);
   // splits: enough workgroups for the CUs, of at least 256 keys
   const long long cap = (long long)C.stride << C.shift;
   long long len = max_len > 0 ? max_len : 4096;
@@ -775,15 +878,15 @@ int launch(lt_ctx* ctx, const AttnArgs& A, const Plan& P) {
   constexpr int KT = F16 ? 32 : 16, KT2 = F16 && HDP <= 128 ? 64 : KT, KW = 2, NT = HDP <= 128 ? 2 : 1;
   switch (P.form) {
     case kDecode16:
-      return go(k_attn_paged<HDP, 1, 1, KW, KT, F16, 1>, 64 * KW, Cfg<HDP, 1, 1, KW, KT, F16>::kLds);
+      return go(k_attn_paged<HDP, 1, 1, KW, KT, F16, 1, true>, 64 * KW, Cfg<HDP, 1, 1, KW, KT, F16>::kLds);
     case kDecode32:
-      if constexpr (HDP <= 128) return go(k_attn_paged<HDP, 2, 1, KW, KT, F16, 1>, 64 * KW, Cfg<HDP, 2, 1, KW, KT, F16>::kLds);
+      if constexpr (HDP <= 128) return go(k_attn_paged<HDP, 2, 1, KW, KT, F16, 1, true>, 64 * KW, Cfg<HDP, 2, 1, KW, KT, F16>::kLds);
       break;
     case kRows64:
-      if constexpr (HDP <= 128) return go(k_attn_paged<HDP, 2, 2, 2, KT, F16, 1>, 256, Cfg<HDP, 2, 2, 2, KT, F16>::kLds);
+      if constexpr (HDP <= 128) return go(k_attn_paged<HDP, 2, 2, 2, KT, F16, 1, false>, 256, Cfg<HDP, 2, 2, 2, KT, F16>::kLds);
       break;
     case kRows128:
-      return go(k_attn_paged<HDP, NT, 4, 1, KT2, F16, 2>, 256, Cfg<HDP, NT, 4, 1, KT2, F16>::kLds);
+      return go(k_attn_paged<HDP, NT, 4, 1, KT2, F16, 2, false>, 256, Cfg<HDP, NT, 4, 1, KT2, F16>::kLds);
   }
   return lt_fail(LT_EINVAL, "lt_attn_paged: no kernel");
 }
@@ -826,7 +929,8 @@ int lt_attn_paged(lt_ctx* ctx, const float* q, int q_stride, int T, const int* q
   if (T == 0) return LT_OK;
   const LtDeviceGuard guard(ctx);
   AttnArgs A = {q, q_stride, q_start, len, B, T, nh, nh / C.nkv, C, out, scale < 0 ? -scale : scale, scale < 0 ? -1.0f : 1.0f,
-                window, err, lt_aligned(q, 16) && q_stride % 4 == 0 && lt_aligned(out, 16), P.chunk, P.nsplit, {}};
+                window, err, lt_aligned(q, 16) && q_stride % 4 == 0 && lt_aligned(out, 16), P.chunk, P.nsplit, {},
+                make_div(nh / C.nkv), make_div(P.chunk ? P.chunk : 1), make_div(C.nkv), make_div(nh)};
   if (P.nsplit > 1) A.ws = lt_attn_ws_layout(ws, T * nh, C.hd, P.nsplit);
   int rc;
   if (C.hd <= 64) rc = f16 ? launch<64, true>(ctx, A, P) : launch<64, false>(ctx, A, P);
