@@ -30,7 +30,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // P is held as 2^7 exp2(score - reference), the reference moved once a score passes it by 8: at most 2^15, and a weight
 // of 2^-32 of the largest still has a term
 constexpr float kPShift = 7.0f, kSlack = 8.0f;
-constexpr int kMaxSplits = 128;
+constexpr int kMaxSplits = 128, kCus = 256;
 
 __device__ const u32x4 g_zero16 = {0, 0, 0, 0};   // what a row without a page reads
 
@@ -858,7 +858,7 @@ Plan make_plan(int T, int B, int nh, const PagedKv& C, bool f16, int max_q, int 
   if (len > cap) len = cap;
   if (window > 0 && len > (long long)window + max_q) len = (long long)window + max_q;
   const long long est = (full > seqs ? full : seqs) * C.nkv;
-  long long want = (512 + est - 1) / est;
+  long long want = !P.per_seq ? (2 * kCus + est - 1) / est : est >= kCus ? 1 : kCus / est;
   if (want > kMaxSplits) want = kMaxSplits;
   long long chunk = (len + want - 1) / want;
   if (chunk < 256) chunk = 256;
@@ -875,15 +875,15 @@ int launch(lt_ctx* ctx, const AttnArgs& A, const Plan& P) {
     kernel<<<grid, threads, lds, ctx->stream>>>(A);
     return lt_check_launch("k_attn_paged");
   };
-  constexpr int KT = F16 ? 32 : 16, KT2 = F16 && HDP <= 128 ? 64 : KT, KW = 2, NT = HDP <= 128 ? 2 : 1;
+  constexpr int KT = F16 ? 32 : 16, KT2 = F16 && HDP <= 128 ? 64 : KT, KW = HDP <= 128 ? 4 : 2, NT = HDP <= 128 ? 2 : 1;
   switch (P.form) {
     case kDecode16:
       return go(k_attn_paged<HDP, 1, 1, KW, KT, F16, 1, true>, 64 * KW, Cfg<HDP, 1, 1, KW, KT, F16>::kLds);
     case kDecode32:
-      if constexpr (HDP <= 128) return go(k_attn_paged<HDP, 2, 1, KW, KT, F16, 1, true>, 64 * KW, Cfg<HDP, 2, 1, KW, KT, F16>::kLds);
+      if constexpr (HDP <= 128) return go(k_attn_paged<HDP, 1, 2, 4, KT, F16, 1, true>, 512, Cfg<HDP, 1, 2, 4, KT, F16>::kLds);
       break;
     case kRows64:
-      if constexpr (HDP <= 128) return go(k_attn_paged<HDP, 2, 2, 2, KT, F16, 1, false>, 256, Cfg<HDP, 2, 2, 2, KT, F16>::kLds);
+      if constexpr (HDP <= 128) return go(k_attn_paged<HDP, 1, 4, 2, KT, F16, 1, false>, 512, Cfg<HDP, 1, 4, 2, KT, F16>::kLds);
       break;
     case kRows128:
       return go(k_attn_paged<HDP, NT, 4, 1, KT2, F16, 2, false>, 256, Cfg<HDP, NT, 4, 1, KT2, F16>::kLds);
