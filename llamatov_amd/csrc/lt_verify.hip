@@ -14,11 +14,12 @@
 // from P alone.  Weights and sums are binary64: the result is a choice of whole numbers, and a binary32 sum of
 // 1024 weights would move a boundary by 1e-7 of the mass.
 //
-// Three launches.  (1) k_verify_slices: the candidates of each slice of each row -- the logits are read once,
-// into registers; the k-th largest of the threads' maxima bounds the slice's k-th largest from below, so the
-// radix select runs over the few keys past that bound.  (2) k_verify_rows: one workgroup a row merges its
-// slices, sorts, and writes the distribution and the probability of the row's draft.  (3) k_verify_seqs: one
-// workgroup a sequence finds the first draft not accepted and draws the last token.
+// Three launches.  (1) k_verify_maxima reads the logits once and keeps the largest of each group of 4 to 64
+// neighbours: the work of a pass over memory.  (2) k_verify_rows, one workgroup a row: the k groups with the
+// largest maxima (ties to the lower group) hold the k largest logits -- any other group's logits have k larger ones, one
+// in each of those -- and of them only those not below the k-th maximum, so that little more than k logits are read
+// again, sorted, and turned into the distribution and the probability of the row's draft.  (3) k_verify_seqs, one
+// workgroup a sequence: the first draft not accepted, and the last token.
 #include "lt_internal.h"
 #include "lt_q8_device.h"
 #include "lt_select.h"
@@ -28,16 +29,18 @@ using namespace lt;
 
 namespace {
 
-constexpr int kVfMaxSlices = 32;                    // 262144 logits in slices of 8192
+constexpr int kVfMaxV = 262144;
+constexpr int kVfGroups = 4 * kSmThreads;           // groups of a row at most: four a thread
+constexpr int kVfCand = 4 * kSmThreads;             // logits not below the bound that LDS holds
+constexpr int kVfSpan = 8192;                       // logits of a workgroup of k_verify_maxima
 typedef unsigned long long u64;
 
 struct VfWs {
-  u64* cand;     // [rows][slices][kSmMaxK] (order key << 32) | ~index
   double* p;     // [rows][kSmMaxK] probabilities in rank order
   double* px;    // [rows] probability of the row's draft
   int* id;       // [rows][kSmMaxK]
   int* n;        // [rows] candidates with a probability
-  int* cnt;      // [rows][slices]
+  uint32_t* top; // [rows][groups] largest order key of each group
 };
 
 struct VfArgs {
@@ -47,7 +50,7 @@ struct VfArgs {
   const int* q_start;
   const float* u;
   lt_sample_params* params;
-  int B, T, V, slices;
+  int B, T, V, group, groups;
   int* out_tok;
   int* n_out;
   int* len;
@@ -66,70 +69,48 @@ __device__ const float* vf_row(const VfArgs& A, int row, int* b, int* draft) {
   return last ? nullptr : A.dlogits + (size_t)r * A.V;
 }
 
-template <int PER>
-__global__ __launch_bounds__(kSmThreads) void k_verify_slices(VfArgs A) {
-  __shared__ SmShared S;
-  const int row = blockIdx.y, sl = blockIdx.x, t = threadIdx.x;
+// Largest order keys of groups of GROUP neighbouring logits.  VEC: rows of whole 16-byte words, four logits a lane.
+template <int GROUP, bool VEC>
+__global__ __launch_bounds__(256) void k_verify_maxima(VfArgs A) {
   int b, draft;
-  const float* l = vf_row(A, row, &b, &draft);
+  const float* l = vf_row(A, blockIdx.y, &b, &draft);
   if (!l) return;
-  const int base = sl * PER * kSmThreads;
-  const int nvalid = A.V - base < PER * kSmThreads ? A.V - base : PER * kSmThreads;
-  int k = sample_k(A.params + b, A.V);
-  if (k > nvalid) k = nvalid;
-  uint32_t key[PER];
-  bool live[PER];
-  float v[PER];
+  constexpr int PER = VEC ? 4 : 1, U = 8, LANES = GROUP / PER;   // lanes of a group
+  uint32_t* top = A.ws.top + (size_t)blockIdx.y * A.groups;
+  for (int base = blockIdx.x * kVfSpan; base < (blockIdx.x + 1) * kVfSpan; base += 256 * PER * U) {
+    uint32_t key[U];
+    float v[U][PER];
 #pragma unroll
-  for (int j = 0; j < PER; j++) {
-    live[j] = j * kSmThreads + t < nvalid;
-    v[j] = live[j] ? l[base + j * kSmThreads + t] : 0.0f;
+    for (int u = 0; u < U; u++) {
+      const int i = base + (u * 256 + threadIdx.x) * PER;
+      if constexpr (VEC) {
+        const float4 x = i < A.V ? *(const float4*)(l + i) : make_float4(0, 0, 0, 0);
+        v[u][0] = x.x;
+        v[u][1] = x.y;
+        v[u][2] = x.z;
+        v[u][3] = x.w;
+      } else {
+        v[u][0] = i < A.V ? l[i] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = base + (u * 256 + threadIdx.x) * PER;
+      key[u] = order_key(v[u][0]);
+#pragma unroll
+      for (int j = 1; j < PER; j++) {
+        const uint32_t kj = order_key(v[u][j]);
+        key[u] = kj > key[u] ? kj : key[u];
+      }
+      if (i >= A.V) key[u] = 0u;   // below or level with every logit's
+#pragma unroll
+      for (int o = 1; o < LANES; o <<= 1) {
+        const uint32_t y = __shfl_xor(key[u], o, 64);
+        key[u] = y > key[u] ? y : key[u];
+      }
+      if ((threadIdx.x & (LANES - 1)) == 0 && i < A.V) top[i / GROUP] = key[u];
+    }
   }
-  uint32_t top[1] = {0u};
-#pragma unroll
-  for (int j = 0; j < PER; j++) {
-    key[j] = order_key(v[j]);
-    if (live[j] && key[j] > top[0]) top[0] = key[j];
-  }
-  // k <= min(threads with a logit, nvalid): at least k keys are at or above the k-th largest maximum
-  const bool any[1] = {live[0]};
-  int rem;
-  const uint32_t bound = radix_select<1>(top, any, k, S, &rem);
-#pragma unroll
-  for (int j = 0; j < PER; j++) live[j] = live[j] && key[j] >= bound;
-  const uint32_t thr = radix_select<PER>(key, live, k, S, &rem);
-  // keys equal to thr: all of them, or (when the tie straddles rank k) the rem lowest indices
-  bool eq[PER];
-  int neq = 0;
-#pragma unroll
-  for (int j = 0; j < PER; j++) {
-    eq[j] = live[j] && key[j] == thr;
-    neq += eq[j];
-  }
-  int eq_total;
-  (void)block_excl_scan(neq, S, &eq_total);
-  uint32_t nthr = 0u;
-  if (eq_total > rem) {
-    uint32_t nidx[PER];
-#pragma unroll
-    for (int j = 0; j < PER; j++) nidx[j] = ~(uint32_t)(base + j * kSmThreads + t);
-    int rem2;
-    nthr = radix_select<PER>(nidx, eq, rem, S, &rem2);
-  }
-  int nsel = 0;
-#pragma unroll
-  for (int j = 0; j < PER; j++) {
-    live[j] = live[j] && (key[j] > thr || (eq[j] && ~(uint32_t)(base + j * kSmThreads + t) >= nthr));
-    nsel += live[j];
-  }
-  int total;
-  int o = block_excl_scan(nsel, S, &total);
-  const size_t at = (size_t)row * A.slices + sl;
-  u64* out = A.ws.cand + at * kSmMaxK;
-#pragma unroll
-  for (int j = 0; j < PER; j++)
-    if (live[j]) out[o++] = ((u64)key[j] << 32) | (uint32_t)~(uint32_t)(base + j * kSmThreads + t);
-  if (t == 0) A.ws.cnt[at] = k;
 }
 
 // Inclusive prefix sum of x over the threads in thread order; *total gets the sum.
@@ -154,74 +135,162 @@ __device__ double scan_f64(double x, double* wave_sum, double* total) {
   return before + x;
 }
 
-template <int NS>   // slices at most
+// Calls f(pair, valid) for the logits of the selected groups, every lane of a wave together; pair orders logits by
+// rank, (order key << 32) | ~index.
+template <class F>
+__device__ __forceinline__ void vf_each(const VfArgs& A, const float* l, const int* grp, int count, F f) {
+  const int per = 64 / A.group;            // groups of a wave's load
+  const int in = threadIdx.x & (A.group - 1), sub = (threadIdx.x & 63) / A.group;
+  constexpr int U = 4;
+  for (int g = (threadIdx.x >> 6) * per; g < count; g += kSmWaves * per * U) {
+    float v[U];
+    int idx[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int gi = g + u * kSmWaves * per + sub;
+      idx[u] = gi < count ? grp[gi] * A.group + in : A.V;
+      v[u] = idx[u] < A.V ? l[idx[u]] : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) f(((u64)order_key(v[u]) << 32) | (uint32_t)~(uint32_t)idx[u], idx[u] < A.V);
+  }
+}
+
 __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
   __shared__ SmShared S;
-  __shared__ u64 s_key[kSmMaxK];
+  __shared__ u64 s_key[kVfCand];
+  __shared__ int s_grp[kSmMaxK];
   __shared__ double s_sum[kSmWaves];
   __shared__ double s_c[kSmMaxK];
   __shared__ double s_px;
-  __shared__ int s_n;
+  __shared__ int s_n, s_count;
   const int row = blockIdx.x, t = threadIdx.x;
   int b, draft;
-  if (!vf_row(A, row, &b, &draft)) return;
+  const float* l = vf_row(A, row, &b, &draft);
+  if (!l) return;
   const lt_sample_params* P = A.params + b;
   const int kc = sample_k(P, A.V);
-  int cnt[NS];
-  int M = 0;
+  // the kc groups of the largest maxima (all groups, if there are no more)
+  uint32_t bound = 0u;
+  int count;
+  {
+    uint32_t key[4];
+    bool live[4];
+    const uint32_t* top = A.ws.top + (size_t)row * A.groups;
 #pragma unroll
-  for (int r = 0; r < NS; r++) {
-    cnt[r] = r < A.slices ? A.ws.cnt[(size_t)row * A.slices + r] : 0;
-    M += cnt[r];
+    for (int j = 0; j < 4; j++) {
+      live[j] = j * kSmThreads + t < A.groups;
+      key[j] = live[j] ? top[j * kSmThreads + t] : 0u;
+    }
+    if (t == 0) s_count = 0;
+    if (A.groups > kc) {
+      int rem;
+      bound = radix_select<4>(key, live, kc, S, &rem);
+      bool eq[4];
+      int neq = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        eq[j] = live[j] && key[j] == bound;
+        neq += eq[j];
+      }
+      int eq_total;
+      (void)block_excl_scan(neq, S, &eq_total);
+      uint32_t last = 0u;   // ties at the bound: the rem lowest groups
+      if (eq_total > rem) {
+        uint32_t ng[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) ng[j] = ~(uint32_t)(j * kSmThreads + t);
+        int rem2;
+        last = radix_select<4>(ng, eq, rem, S, &rem2);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        live[j] = live[j] && (key[j] > bound || (eq[j] && ~(uint32_t)(j * kSmThreads + t) >= last));
+    }
+    int sel = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) sel += live[j];
+    int o = block_excl_scan(sel, S, &count);
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (live[j]) s_grp[o++] = j * kSmThreads + t;
+    __syncthreads();
   }
-  const u64* cand = A.ws.cand + (size_t)row * A.slices * kSmMaxK;
+  // their logits at or above the bound, in any order (the sort settles it)
+  auto gather = [&](u64 least) {
+    vf_each(A, l, s_grp, count, [&](u64 pair, bool on) {
+      on = on && pair >= least;
+      const u64 m = __ballot(on);
+      if (!m) return;
+      int at = 0;
+      if ((t & 63) == 0) at = atomicAdd(&s_count, (int)__popcll(m));
+      at = __builtin_amdgcn_readfirstlane(at) + (int)__popcll(m & ((1ull << (t & 63)) - 1));
+      if (on && at < kVfCand) s_key[at] = pair;
+    });
+    __syncthreads();
+    return s_count;
+  };
+  int M = gather((u64)bound << 32);
+  if (M > kVfCand) {
+    // too many of them (runs of large neighbours): the kc-th pair itself, digit by digit over the groups' logits
+    u64 prefix = 0ull, mask = 0ull;
+    int rem = kc;
+#pragma unroll 1
+    for (int shift = 56; shift >= 0; shift -= 8) {
+      if (t < 256) S.hist[t] = 0;
+      __syncthreads();
+      vf_each(A, l, s_grp, count, [&](u64 pair, bool on) {
+        if (on && (pair & mask) == prefix) atomicAdd(&S.hist[(int)(pair >> shift) & 255], 1);
+      });
+      __syncthreads();
+      if (t < 64) find_digit(S, rem);
+      __syncthreads();
+      prefix |= (u64)S.sel_digit << shift;
+      mask |= 255ull << shift;
+      rem = S.sel_rem;
+    }
+    if (t == 0) s_count = 0;
+    __syncthreads();
+    M = gather(prefix);
+  }
   int P2 = 1;
   u64 x = 0ull;   // padding: below every candidate
   if (M <= kSmThreads) {
-    // thread t takes the t-th candidate in slice order
     while (P2 < M) P2 <<= 1;
-    int r = 0, before = 0, end = 0;
-#pragma unroll
-    for (int q = 0; q < NS; q++) {
-      end += cnt[q];
-      if (end <= t) {
-        r = q + 1;
-        before = end;
-      }
-    }
-    if (t < M) x = cand[(size_t)r * kSmMaxK + (t - before)];
+    if (t < M) x = s_key[t];
+    __syncthreads();
   } else {
     // the first kc of them by a radix select, ties at the threshold by index
-    uint32_t key[NS], nidx[NS];
-    bool live[NS];
+    uint32_t key[4], nidx[4];
+    bool live[4];
 #pragma unroll
-    for (int r = 0; r < NS; r++) {
-      live[r] = t < cnt[r];
-      const u64 c = live[r] ? cand[(size_t)r * kSmMaxK + t] : 0ull;
-      key[r] = (uint32_t)(c >> 32);
-      nidx[r] = (uint32_t)c;
+    for (int j = 0; j < 4; j++) {
+      live[j] = j * kSmThreads + t < M;
+      const u64 c = live[j] ? s_key[j * kSmThreads + t] : 0ull;
+      key[j] = (uint32_t)(c >> 32);
+      nidx[j] = (uint32_t)c;
     }
     int rem;
-    const uint32_t thr = radix_select<NS>(key, live, kc, S, &rem);
-    bool eq[NS];
+    const uint32_t thr = radix_select<4>(key, live, kc, S, &rem);
+    bool eq[4];
     int neq = 0;
 #pragma unroll
-    for (int r = 0; r < NS; r++) {
-      eq[r] = live[r] && key[r] == thr;
-      neq += eq[r];
+    for (int j = 0; j < 4; j++) {
+      eq[j] = live[j] && key[j] == thr;
+      neq += eq[j];
     }
     int eq_total;
     (void)block_excl_scan(neq, S, &eq_total);
     uint32_t nthr = 0u;
     if (eq_total > rem) {
       int rem2;
-      nthr = radix_select<NS>(nidx, eq, rem, S, &rem2);
+      nthr = radix_select<4>(nidx, eq, rem, S, &rem2);
     }
     int nsel = 0;
 #pragma unroll
-    for (int r = 0; r < NS; r++) {
-      live[r] = live[r] && (key[r] > thr || (eq[r] && nidx[r] >= nthr));
-      nsel += live[r];
+    for (int j = 0; j < 4; j++) {
+      live[j] = live[j] && (key[j] > thr || (eq[j] && nidx[j] >= nthr));
+      nsel += live[j];
     }
     int total;
     int o = block_excl_scan(nsel, S, &total);
@@ -229,8 +298,8 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
     s_key[t] = 0ull;
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < NS; r++)
-      if (live[r]) s_key[o++] = ((u64)key[r] << 32) | nidx[r];
+    for (int j = 0; j < 4; j++)
+      if (live[j]) s_key[o++] = ((u64)key[j] << 32) | nidx[j];
     __syncthreads();
     x = s_key[t];
     __syncthreads();
@@ -355,26 +424,32 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_seqs(VfArgs A) {
   }
 }
 
-// Logits a thread holds: 32 when that leaves at least two workgroups a CU, else 8 (more workgroups).
-int vf_per(int rows, int V) { return (long long)rows * ((V + 32767) / 32768) >= 512 ? 32 : 8; }
+// Neighbours of a group: at most kVfGroups groups a row, and many more than the 1024 that a row may select.
+int vf_group(int V) { return V <= 4 * kVfGroups ? 4 : V <= 16 * kVfGroups ? 16 : V <= 32 * kVfGroups ? 32 : 64; }
 
-int vf_slices(int rows, int V) {
-  const int n = vf_per(rows, V) * kSmThreads;
-  return (V + n - 1) / n;
-}
+int vf_groups(int V) { return (V + vf_group(V) - 1) / vf_group(V); }
 
-VfWs vf_layout(void* ws, int rows, int slices) {
+VfWs vf_layout(void* ws, int rows, int groups) {
   VfWs w;
-  w.cand = (u64*)ws;
-  w.p = (double*)(w.cand + (size_t)rows * slices * kSmMaxK);
+  w.p = (double*)ws;
   w.px = w.p + (size_t)rows * kSmMaxK;
   w.id = (int*)(w.px + rows);
   w.n = w.id + (size_t)rows * kSmMaxK;
-  w.cnt = w.n + rows;
+  w.top = (uint32_t*)(w.n + rows);
   return w;
 }
 
-bool vf_sizes(int T, int V) { return T >= 0 && T <= 32767 && V > 0 && V <= kVfMaxSlices * 8 * kSmThreads; }
+bool vf_sizes(int T, int V) { return T >= 0 && T <= 32767 && V > 0 && V <= kVfMaxV; }
+
+template <bool VEC>
+void vf_maxima(const VfArgs& A, dim3 grid, hipStream_t stream) {
+  switch (A.group) {
+    case 4: k_verify_maxima<4, VEC><<<grid, 256, 0, stream>>>(A); break;
+    case 16: k_verify_maxima<16, VEC><<<grid, 256, 0, stream>>>(A); break;
+    case 32: k_verify_maxima<32, VEC><<<grid, 256, 0, stream>>>(A); break;
+    default: k_verify_maxima<64, VEC><<<grid, 256, 0, stream>>>(A); break;
+  }
+}
 
 }  // namespace
 
@@ -383,9 +458,7 @@ extern "C" {
 size_t lt_verify_drafts_workspace_size(int T, int V, int drafter) {
   if (!vf_sizes(T, V)) return 0;
   const int rows = drafter ? 2 * T : T;
-  const size_t per_row = (size_t)vf_slices(rows, V) * (kSmMaxK * sizeof(u64) + sizeof(int)) +
-                         kSmMaxK * (sizeof(double) + sizeof(int)) + sizeof(double) + sizeof(int);
-  return rows * per_row;
+  return rows * (kSmMaxK * (sizeof(double) + sizeof(int)) + sizeof(double) + sizeof(int) + vf_groups(V) * sizeof(uint32_t));
 }
 
 int lt_verify_drafts(lt_ctx* ctx, const float* logits, const float* draft_logits, const int* toks,
@@ -393,7 +466,7 @@ int lt_verify_drafts(lt_ctx* ctx, const float* logits, const float* draft_logits
                      int* out_tok, int* n_out, int* len, void* ws, size_t ws_bytes) {
   LT_REQUIRE(logits && toks && q_start && params && out_tok && n_out && ws, "lt_verify_drafts: null argument");
   LT_REQUIRE(B > 0 && B <= 65535 && vf_sizes(T, V), "lt_verify_drafts: B=%d (1 .. 65535) T=%d (0 .. 32767) V=%d (1 .. %d)",
-             B, T, V, kVfMaxSlices * 8 * kSmThreads);
+             B, T, V, kVfMaxV);
   LT_REQUIRE(lt_aligned(params, 8) && lt_aligned(ws, 8) && lt_aligned(logits, 4) && lt_aligned(draft_logits, 4),
              "lt_verify_drafts: params and ws 8-byte, logits 4-byte aligned");
   const size_t need = lt_verify_drafts_workspace_size(T, V, draft_logits != nullptr);
@@ -402,19 +475,14 @@ int lt_verify_drafts(lt_ctx* ctx, const float* logits, const float* draft_logits
   LT_REQUIRE(ctx, "lt_verify_drafts: null ctx");
   const LtDeviceGuard guard(ctx);
   const int rows = draft_logits ? 2 * T : T;
-  const int slices = vf_slices(rows ? rows : 1, V);
-  const VfArgs A = {logits, draft_logits, toks, q_start, u, params, B, T, V, slices, out_tok, n_out, len,
-                    vf_layout(ws, rows, slices)};
+  const VfArgs A = {logits, draft_logits, toks, q_start, u, params, B, T, V, vf_group(V), vf_groups(V), out_tok, n_out,
+                    len, vf_layout(ws, rows, vf_groups(V))};
   if (rows) {
-    if (vf_per(rows, V) == 32)
-      k_verify_slices<32><<<dim3(slices, rows), kSmThreads, 0, ctx->stream>>>(A);
-    else
-      k_verify_slices<8><<<dim3(slices, rows), kSmThreads, 0, ctx->stream>>>(A);
-    if (int rc = lt_check_launch("k_verify_slices")) return rc;
-    if (slices <= 8)
-      k_verify_rows<8><<<rows, kSmThreads, 0, ctx->stream>>>(A);
-    else
-      k_verify_rows<kVfMaxSlices><<<rows, kSmThreads, 0, ctx->stream>>>(A);
+    const dim3 grid((V + kVfSpan - 1) / kVfSpan, rows);
+    if (V % 4 == 0 && lt_aligned(logits, 16) && lt_aligned(draft_logits, 16)) vf_maxima<true>(A, grid, ctx->stream);
+    else vf_maxima<false>(A, grid, ctx->stream);
+    if (int rc = lt_check_launch("k_verify_maxima")) return rc;
+    k_verify_rows<<<rows, kSmThreads, 0, ctx->stream>>>(A);
     if (int rc = lt_check_launch("k_verify_rows")) return rc;
   }
   k_verify_seqs<<<B, kSmThreads, 0, ctx->stream>>>(A);

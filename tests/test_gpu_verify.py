@@ -158,6 +158,29 @@ def test_verification_large_batch(gpu, V):
     assert np.array_equal(n, en) and np.array_equal(out, eo)
 
 
+@pytest.mark.parametrize("V", [4100, 16384, 16387, 65540, 131072, 200001])
+def test_verification_runs_of_large_neighbours(gpu, V):
+    """Logits in ascending, descending and equal order, and blocks of equal large ones: far more of them at or above the
+    bound of the groups than are candidates."""
+    case(f"verify runs V={V}")
+    rng = np.random.default_rng(V)
+    settings = [(1.0, 1024, 1.0), (0.7, 40, 0.9), (1.0, 1000, 0.99)]
+    b = batch(rng, V, [3, 3, 3, 3, 2], settings, True)
+    for l in (b[0], b[1]):
+        up = (np.arange(V) * np.float32(2e-4)).astype(np.float32)
+        l[0:3] = up
+        l[3:6] = up[::-1]
+        l[6:9] = 1.5
+        l[9:12, V // 3:V // 3 + 3000] = 9.0
+        l[9, V - 1] = 9.5
+        l[12:, :4000] = np.floor(up[:4000] * 50)
+    toks = b[2]
+    toks[1], toks[4], toks[7], toks[10], toks[13] = V - 3, 2, 5, V // 3 + 7, 3999
+    out, n, _, _ = run(gpu, *b)
+    eo, en = verify(*b)
+    assert np.array_equal(n, en) and np.array_equal(out, eo)
+
+
 def test_verification_agreeing_drafter_accepts_all(gpu):
     case("verify equal logits")
     rng = np.random.default_rng(5)
