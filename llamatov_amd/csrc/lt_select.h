@@ -92,8 +92,9 @@ static __device__ void find_digit(SmShared& S, int rem) {
 }
 
 // Radix select over N keys per thread (those with live[j]): returns the key T of rank `rem`
-// (1 = largest) among them and sets *rem_out to T's rank among the keys equal to T.
-template <int N>
+// (1 = largest) among them and sets *rem_out to T's rank among the keys equal to T.  BYTES < 4: only the
+// leading bytes of T are found and *rem_out is its rank among the keys that share them.
+template <int N, int BYTES = 4>
 __device__ uint32_t radix_select(const uint32_t (&key)[N], const bool (&live)[N], int rem, SmShared& S,
                                  int* rem_out) {
   uint32_t prefix = 0, mask = 0;
@@ -118,7 +119,7 @@ __device__ uint32_t radix_select(const uint32_t (&key)[N], const bool (&live)[N]
     S.hist[threadIdx.x] = c;
   }
 #pragma unroll 1
-  for (int pass = 0; pass < 4; pass++) {
+  for (int pass = 0; pass < BYTES; pass++) {
     const int shift = 24 - 8 * pass;
     if (pass > 0) {
       if (threadIdx.x < 256) S.hist[threadIdx.x] = 0;

@@ -15,11 +15,13 @@
 // 1024 weights would move a boundary by 1e-7 of the mass.
 //
 // Three launches.  (1) k_verify_maxima reads the logits once and keeps the largest of each group of 4 to 64
-// neighbours: the work of a pass over memory.  (2) k_verify_rows, one workgroup a row: the k groups with the
-// largest maxima (ties to the lower group) hold the k largest logits -- any other group's logits have k larger ones, one
-// in each of those -- and of them only those not below the k-th maximum, so that little more than k logits are read
-// again, sorted, and turned into the distribution and the probability of the row's draft.  (3) k_verify_seqs, one
+// neighbours: the work of a pass over memory.  (2) k_verify_rows, one workgroup a row: k groups have a
+// maximum at or above the k-th largest of the maxima, so the k largest logits are not below that one and lie in groups
+// whose maxima are not either; little more than k logits are read again, sorted, and turned into the distribution and
+// the probability of the row's draft.  The k-th maximum's leading 16 bits are bound enough.  (3) k_verify_seqs, one
 // workgroup a sequence: the first draft not accepted, and the last token.
+#include <type_traits>
+
 #include "lt_internal.h"
 #include "lt_q8_device.h"
 #include "lt_select.h"
@@ -135,31 +137,75 @@ __device__ double scan_f64(double x, double* wave_sum, double* total) {
   return before + x;
 }
 
-// Calls f(pair, valid) for the logits of the selected groups, every lane of a wave together; pair orders logits by
-// rank, (order key << 32) | ~index.
-template <class F>
+// Calls f(pairs, valid) for the logits of the selected groups, U * PER of them a lane and every lane of a wave together;
+// pairs order logits by rank, (order key << 32) | ~index.
+template <bool VEC, class F>
 __device__ __forceinline__ void vf_each(const VfArgs& A, const float* l, const int* grp, int count, F f) {
-  const int per = 64 / A.group;            // groups of a wave's load
-  const int in = threadIdx.x & (A.group - 1), sub = (threadIdx.x & 63) / A.group;
-  constexpr int U = 4;
+  constexpr int PER = VEC ? 4 : 1, U = VEC ? 4 : 8;
+  const int lanes = A.group / PER;         // lanes of a group
+  const int per = 64 / lanes;              // groups of a wave's load
+  const int in = (threadIdx.x & (lanes - 1)) * PER, sub = (threadIdx.x & 63) / lanes;
   for (int g = (threadIdx.x >> 6) * per; g < count; g += kSmWaves * per * U) {
-    float v[U];
+    float v[U * PER];
     int idx[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int gi = g + u * kSmWaves * per + sub;
       idx[u] = gi < count ? grp[gi] * A.group + in : A.V;
-      v[u] = idx[u] < A.V ? l[idx[u]] : 0.0f;
+      if constexpr (VEC) {
+        const float4 x = idx[u] < A.V ? *(const float4*)(l + idx[u]) : make_float4(0, 0, 0, 0);
+        v[4 * u] = x.x;
+        v[4 * u + 1] = x.y;
+        v[4 * u + 2] = x.z;
+        v[4 * u + 3] = x.w;
+      } else {
+        v[u] = idx[u] < A.V ? l[idx[u]] : 0.0f;
+      }
     }
+    u64 pair[U * PER];
+    bool on[U * PER];
 #pragma unroll
-    for (int u = 0; u < U; u++) f(((u64)order_key(v[u]) << 32) | (uint32_t)~(uint32_t)idx[u], idx[u] < A.V);
+    for (int i = 0; i < U * PER; i++) {
+      pair[i] = ((u64)order_key(v[i]) << 32) | (uint32_t)~(uint32_t)(idx[i / PER] + i % PER);
+      on[i] = idx[i / PER] < A.V;
+    }
+    f(pair, on);
   }
 }
 
+// x of lane ^ S.
+template <int S>
+__device__ __forceinline__ uint32_t xor_lane(uint32_t x) {
+  // quad_perm 1 0 3 2 / 2 3 0 1 / 3 2 1 0, row_half_mirror (lane ^ 7), row_mirror (lane ^ 15)
+  auto dpp = [](uint32_t v, auto ctrl) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, decltype(ctrl)::value, 0xF, 0xF, true);
+  };
+  if constexpr (S == 1) return dpp(x, std::integral_constant<int, 0xB1>{});
+  else if constexpr (S == 2) return dpp(x, std::integral_constant<int, 0x4E>{});
+  else if constexpr (S == 4) return dpp(dpp(x, std::integral_constant<int, 0x1B>{}), std::integral_constant<int, 0x141>{});
+  else if constexpr (S == 8) return dpp(dpp(x, std::integral_constant<int, 0x141>{}), std::integral_constant<int, 0x140>{});
+  else if constexpr (S == 16) {
+    const u32x2 r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return threadIdx.x & 16 ? r.x : r.y;
+  } else {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return threadIdx.x & 32 ? r.x : r.y;
+  }
+}
+
+// One stage of a bitonic network over the lanes of a wave, larger first in descending blocks of `size`.
+template <int S>
+__device__ __forceinline__ u64 sort_stage(u64 x, int size) {
+  const u64 y = (u64)xor_lane<S>((uint32_t)(x >> 32)) << 32 | xor_lane<S>((uint32_t)x);
+  const bool first = ((threadIdx.x & size) == 0) == ((threadIdx.x & S) == 0);
+  return (x > y) == first ? x : y;   // the pairs are distinct, padding apart
+}
+
+template <bool VEC>
 __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
   __shared__ SmShared S;
   __shared__ u64 s_key[kVfCand];
-  __shared__ int s_grp[kSmMaxK];
+  __shared__ int s_grp[kVfGroups];
   __shared__ double s_sum[kSmWaves];
   __shared__ double s_c[kSmMaxK];
   __shared__ double s_px;
@@ -170,7 +216,8 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
   if (!l) return;
   const lt_sample_params* P = A.params + b;
   const int kc = sample_k(P, A.V);
-  // the kc groups of the largest maxima (all groups, if there are no more)
+  // the groups whose maximum is not below the kc-th largest's leading 16 bits, which is a bound for the kc-th largest
+  // logit (all groups, if there are no more than kc)
   uint32_t bound = 0u;
   int count;
   {
@@ -185,27 +232,9 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
     if (t == 0) s_count = 0;
     if (A.groups > kc) {
       int rem;
-      bound = radix_select<4>(key, live, kc, S, &rem);
-      bool eq[4];
-      int neq = 0;
+      bound = radix_select<4, 2>(key, live, kc, S, &rem);
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        eq[j] = live[j] && key[j] == bound;
-        neq += eq[j];
-      }
-      int eq_total;
-      (void)block_excl_scan(neq, S, &eq_total);
-      uint32_t last = 0u;   // ties at the bound: the rem lowest groups
-      if (eq_total > rem) {
-        uint32_t ng[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) ng[j] = ~(uint32_t)(j * kSmThreads + t);
-        int rem2;
-        last = radix_select<4>(ng, eq, rem, S, &rem2);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        live[j] = live[j] && (key[j] > bound || (eq[j] && ~(uint32_t)(j * kSmThreads + t) >= last));
+      for (int j = 0; j < 4; j++) live[j] = live[j] && key[j] >= bound;
     }
     int sel = 0;
 #pragma unroll
@@ -218,14 +247,25 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
   }
   // their logits at or above the bound, in any order (the sort settles it)
   auto gather = [&](u64 least) {
-    vf_each(A, l, s_grp, count, [&](u64 pair, bool on) {
-      on = on && pair >= least;
-      const u64 m = __ballot(on);
-      if (!m) return;
+    vf_each<VEC>(A, l, s_grp, count, [&](auto& pair, auto& on) {
+      constexpr int N = sizeof(on) / sizeof(on[0]);
+      u64 m[N];
+      int total = 0;
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        m[i] = __ballot(on[i] && pair[i] >= least);
+        total += (int)__popcll(m[i]);
+      }
+      if (!total) return;
       int at = 0;
-      if ((t & 63) == 0) at = atomicAdd(&s_count, (int)__popcll(m));
-      at = __builtin_amdgcn_readfirstlane(at) + (int)__popcll(m & ((1ull << (t & 63)) - 1));
-      if (on && at < kVfCand) s_key[at] = pair;
+      if ((t & 63) == 0) at = atomicAdd(&s_count, total);
+      at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const int mine = at + (int)__popcll(m[i] & ((1ull << (t & 63)) - 1));
+        if ((m[i] >> (t & 63) & 1) && mine < kVfCand) s_key[mine] = pair[i];
+        at += (int)__popcll(m[i]);
+      }
     });
     __syncthreads();
     return s_count;
@@ -239,8 +279,10 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
     for (int shift = 56; shift >= 0; shift -= 8) {
       if (t < 256) S.hist[t] = 0;
       __syncthreads();
-      vf_each(A, l, s_grp, count, [&](u64 pair, bool on) {
-        if (on && (pair & mask) == prefix) atomicAdd(&S.hist[(int)(pair >> shift) & 255], 1);
+      vf_each<VEC>(A, l, s_grp, count, [&](auto& pair, auto& on) {
+        constexpr int N = sizeof(on) / sizeof(on[0]);
+        for (int i = 0; i < N; i++)
+          if (on[i] && (pair[i] & mask) == prefix) atomicAdd(&S.hist[(int)(pair[i] >> shift) & 255], 1);
       });
       __syncthreads();
       if (t < 64) find_digit(S, rem);
@@ -304,22 +346,27 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
     x = s_key[t];
     __syncthreads();
   }
-  // bitonic network, larger first, one key a thread; partners in the same wave trade by shuffles
-  if (P2 > 64 || t < 64)
-    for (int size = 2; size <= P2; size <<= 1)
-      for (int stride = size >> 1; stride > 0; stride >>= 1) {
-        u64 y;
-        if (stride >= 64) {
-          s_key[t] = x;
-          __syncthreads();
-          y = s_key[t ^ stride];
-          __syncthreads();
-        } else {
-          y = __shfl_xor(x, stride, 64);
-        }
+  // bitonic network, larger first, one key a thread; partners in other waves trade through LDS, in two halves in turn
+  if (P2 > 64 || t < 64) {
+    int half = 0;
+    for (int size = 2; size <= P2; size <<= 1) {
+      for (int stride = size >> 1; stride >= 64; stride >>= 1) {
+        s_key[half + t] = x;
+        __syncthreads();
+        const u64 y = s_key[half + (t ^ stride)];
+        half ^= kSmThreads;
         const bool first = ((t & size) == 0) == ((t & stride) == 0);
-        x = first ? (x > y ? x : y) : (x > y ? y : x);
+        x = (x > y) == first ? x : y;
       }
+      if (size >= 64) x = sort_stage<32>(x, size);
+      if (size >= 32) x = sort_stage<16>(x, size);
+      if (size >= 16) x = sort_stage<8>(x, size);
+      if (size >= 8) x = sort_stage<4>(x, size);
+      if (size >= 4) x = sort_stage<2>(x, size);
+      x = sort_stage<1>(x, size);
+    }
+  }
+  __syncthreads();
   if (t == 0) {
     s_key[0] = x;
     s_px = 0.0;
@@ -336,7 +383,10 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
   s_c[t] = c;
   __syncthreads();
   const float topp = P->top_p;
-  if (topp < 1.0f && t < k && c >= (double)topp * s_c[k - 1]) atomicMin(&s_n, t + 1);
+  if (topp < 1.0f) {
+    const u64 hit = __ballot(t < k && c >= (double)topp * s_c[k - 1]);
+    if (hit && (t & 63) == __builtin_ctzll(hit)) atomicMin(&s_n, t + 1);
+  }
   __syncthreads();
   const int n = s_n;
   const int id = (int)~(uint32_t)x;
@@ -355,13 +405,40 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
 
 // A row's candidates: within the list's room whatever the workspace holds (a row that q_start gives to two
 // sequences may have been skipped).
-__device__ __forceinline__ int vf_count(const VfArgs& A, int row) {
-  const int n = A.ws.n[row];
-  return n < 0 ? 0 : n < kSmMaxK ? n : kSmMaxK;
+__device__ __forceinline__ int vf_count(int n) { return n < 0 ? 0 : n < kSmMaxK ? n : kSmMaxK; }
+
+constexpr int kSeqThreads = 256, kSeqWaves = kSeqThreads / 64, kSeqPer = kSmMaxK / kSeqThreads;
+
+// Inclusive prefix sums of four values a thread, in thread order; *total gets the sum.
+__device__ __forceinline__ void scan4_f64(const double (&w)[kSeqPer], double (&c)[kSeqPer], double* wave_sum, double* total) {
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  c[0] = w[0];
+#pragma unroll
+  for (int j = 1; j < kSeqPer; j++) c[j] = c[j - 1] + w[j];
+  double x = c[kSeqPer - 1];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();   // wave_sum may still be read from the scan before
+  if (lane == 63) wave_sum[wv] = x;
+  __syncthreads();
+  double before = 0.0, all = 0.0;
+#pragma unroll
+  for (int v = 0; v < kSeqWaves; v++) {
+    if (v < wv) before += wave_sum[v];
+    all += wave_sum[v];
+  }
+  const double up = __shfl_up(x, 1, 64);
+  before += lane ? up : 0.0;
+#pragma unroll
+  for (int j = 0; j < kSeqPer; j++) c[j] += before;
+  *total = all;
 }
 
-__global__ __launch_bounds__(kSmThreads) void k_verify_seqs(VfArgs A) {
-  __shared__ double s_sum[kSmWaves];
+__global__ __launch_bounds__(kSeqThreads) void k_verify_seqs(VfArgs A) {
+  __shared__ double s_sum[kSeqWaves];
   __shared__ double s_q[kSmMaxK];
   __shared__ int s_id[kSmMaxK];
   __shared__ int s_first, s_pick;
@@ -379,44 +456,61 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_seqs(VfArgs A) {
     return (double)(philox_x(P->counter + (u64)i, P->seed) >> 8) * 0x1.0p-24;
   };
   if (t == 0) s_first = rows - 1;
+  const double u_last = uniform(rows - 1);
   __syncthreads();
-  for (int i = t; i < rows - 1; i += kSmThreads) {
+  for (int i = t; i < rows - 1; i += kSeqThreads) {
     const double q = A.dlogits ? A.ws.px[A.T + r0 + i] : 1.0;
     if (!(uniform(i) * q < A.ws.px[r0 + i])) atomicMin(&s_first, i);
   }
   __syncthreads();
   const int first = s_first, r = r0 + first;
-  const bool all = first == rows - 1;
-  const int n = vf_count(A, r);
-  const double p = t < n ? A.ws.p[(size_t)r * kSmMaxK + t] : 0.0;
-  const int id = t < n ? A.ws.id[(size_t)r * kSmMaxK + t] : -1;
-  double w = p;
-  if (!all) {
-    double q = 0.0;
-    if (A.dlogits) {
-      const int nd = vf_count(A, A.T + r);
-      if (t < nd) {
-        s_q[t] = A.ws.p[(size_t)(A.T + r) * kSmMaxK + t];
-        s_id[t] = A.ws.id[(size_t)(A.T + r) * kSmMaxK + t];
-      }
-      __syncthreads();
-      for (int d = 0; d < nd; d++)
-        if (s_id[d] == id) q = s_q[d];
-    } else if (id == A.toks[r + 1]) {
-      q = 1.0;
+  const bool all = first == rows - 1, drafter = !all && A.dlogits;
+  const int n = vf_count(A.ws.n[r]), nd = drafter ? vf_count(A.ws.n[A.T + r]) : 0;
+  const int draft = all ? -1 : A.toks[r + 1];
+  double p[kSeqPer], w[kSeqPer], c[kSeqPer];
+  int id[kSeqPer];
+#pragma unroll
+  for (int j = 0; j < kSeqPer; j++) {
+    const int i = t * kSeqPer + j;
+    p[j] = i < n ? A.ws.p[(size_t)r * kSmMaxK + i] : 0.0;
+    id[j] = i < n ? A.ws.id[(size_t)r * kSmMaxK + i] : -1;
+    // without a drafter's logits Q has all its mass on the draft
+    w[j] = !all && !drafter && id[j] == draft ? 0.0 : p[j];
+  }
+  if (drafter) {
+    for (int i = t; i < nd; i += kSeqThreads) {
+      s_q[i] = A.ws.p[(size_t)(A.T + r) * kSmMaxK + i];
+      s_id[i] = A.ws.id[(size_t)(A.T + r) * kSmMaxK + i];
     }
-    w = p > q ? p - q : 0.0;
+    __syncthreads();
+    int at[kSeqPer] = {-1, -1, -1, -1};
+    for (int d = 0; d < nd; d++) {
+      const int x = s_id[d];
+#pragma unroll
+      for (int j = 0; j < kSeqPer; j++) at[j] = x == id[j] ? d : at[j];
+    }
+#pragma unroll
+    for (int j = 0; j < kSeqPer; j++)
+      if (at[j] >= 0) w[j] = p[j] > s_q[at[j]] ? p[j] - s_q[at[j]] : 0.0;
   }
   double total;
-  double c = scan_f64(w, s_sum, &total);
-  if (!(total > 0.0)) c = scan_f64(p, s_sum, &total);   // nothing is left of P: P itself
+  scan4_f64(w, c, s_sum, &total);
+  if (!(total > 0.0)) scan4_f64(p, c, s_sum, &total);   // nothing is left of P: P itself
   if (t == 0) s_pick = n - 1;
   __syncthreads();
-  if (t < n && c > uniform(rows - 1) * total) atomicMin(&s_pick, t);
+  // the sums do not fall: the first candidate past the goal is the first such lane's first
+  int mine = kSeqPer;
+#pragma unroll
+  for (int j = kSeqPer - 1; j >= 0; j--)
+    if (t * kSeqPer + j < n && c[j] > u_last * total) mine = j;
+  const u64 hit = __ballot(mine < kSeqPer);
+  if (hit && (t & 63) == __builtin_ctzll(hit)) atomicMin(&s_pick, t * kSeqPer + mine);
   __syncthreads();
-  for (int i = t; i < rows; i += kSmThreads)
+  for (int i = t; i < rows; i += kSeqThreads)
     if (i != first) A.out_tok[r0 + i] = i < first ? A.toks[r0 + i + 1] : -1;
-  if (t == s_pick) A.out_tok[r] = id;
+#pragma unroll
+  for (int j = 0; j < kSeqPer; j++)
+    if (t * kSeqPer + j == s_pick) A.out_tok[r] = id[j];
   if (t == 0) {
     A.n_out[b] = first + 1;
     if (A.len) A.len[b] += first + 1;
@@ -479,13 +573,15 @@ int lt_verify_drafts(lt_ctx* ctx, const float* logits, const float* draft_logits
                     len, vf_layout(ws, rows, vf_groups(V))};
   if (rows) {
     const dim3 grid((V + kVfSpan - 1) / kVfSpan, rows);
-    if (V % 4 == 0 && lt_aligned(logits, 16) && lt_aligned(draft_logits, 16)) vf_maxima<true>(A, grid, ctx->stream);
+    const bool vec = V % 4 == 0 && lt_aligned(logits, 16) && lt_aligned(draft_logits, 16);
+    if (vec) vf_maxima<true>(A, grid, ctx->stream);
     else vf_maxima<false>(A, grid, ctx->stream);
     if (int rc = lt_check_launch("k_verify_maxima")) return rc;
-    k_verify_rows<<<rows, kSmThreads, 0, ctx->stream>>>(A);
+    if (vec) k_verify_rows<true><<<rows, kSmThreads, 0, ctx->stream>>>(A);
+    else k_verify_rows<false><<<rows, kSmThreads, 0, ctx->stream>>>(A);
     if (int rc = lt_check_launch("k_verify_rows")) return rc;
   }
-  k_verify_seqs<<<B, kSmThreads, 0, ctx->stream>>>(A);
+  k_verify_seqs<<<B, kSeqThreads, 0, ctx->stream>>>(A);
   return lt_check_launch("k_verify_seqs");
 }
 
