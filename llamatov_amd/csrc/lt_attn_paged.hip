@@ -852,19 +852,20 @@ Plan make_plan(int T, int B, int nh, const PagedKv& C, bool f16, int max_q, int 
   const long long full = (long long)T * rep / P.tm;
   P.per_seq = P.form == kDecode16 || P.form == kDecode32;
   P.tiles = P.per_seq ? B : (int)(full + seqs);
-  // splits: enough workgroups for the CUs, of at least 256 keys
+  // splits: enough workgroups for the CUs (two a CU where registers allow it), of `least` keys at least
   const long long cap = (long long)C.stride << C.shift;
   long long len = max_len > 0 ? max_len : 4096;
   if (len > cap) len = cap;
-  if (window > 0 && len > (long long)window + max_q) len = (long long)window + max_q;
   const long long est = (full > seqs ? full : seqs) * C.nkv;
   long long want = !P.per_seq ? (2 * kCus + est - 1) / est : est >= kCus ? 1 : kCus / est;
   if (want > kMaxSplits) want = kMaxSplits;
+  const long long least = P.per_seq ? 256 : 128, unit = P.per_seq ? 128 : 64;   // unit: the key tiles of all groups
+  P.most = (int)((len + least - 1) / least < want ? (len + least - 1) / least : want);
+  if (window > 0 && len > (long long)window + P.tm / rep + 2) len = (long long)window + P.tm / rep + 2;   // of one tile
   long long chunk = (len + want - 1) / want;
-  if (chunk < 256) chunk = 256;
-  P.chunk = (int)((chunk + 255) / 256 * 256);
+  if (chunk < least) chunk = least;
+  P.chunk = (int)((chunk + unit - 1) / unit * unit);
   P.nsplit = (int)((len + P.chunk - 1) / P.chunk);
-  P.most = (int)((len + 255) / 256 < want ? (len + 255) / 256 : want);
   return P;
 }
 
