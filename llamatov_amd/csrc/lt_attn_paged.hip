@@ -474,6 +474,8 @@ __device__ __forceinline__ bool attend(const AttnArgs& A, const Tile& X, int b, 
   auto compute = [&](int k, int buf, bool masked) {
     uint32_t ka = ka0 + buf * G::kStageB, va = va0 + buf * G::kStageB;
     asm volatile("" : "+v"(ka), "+v"(va));   // the addresses of the steps are formed here, not kept over the loop
+    // waves that share tiles pass their phases together: the workgroup whose products are waiting goes first
+    if (!kOwn) __builtin_amdgcn_s_setprio(2);
     auto k_frag = [&](int c, int m) {
       return *(const __attribute__((address_space(3))) u32x4*)lds((ka ^ (c << 6)) + m * 16 * G::kRowB);
     };
@@ -524,6 +526,7 @@ __device__ __forceinline__ bool attend(const AttnArgs& A, const Tile& X, int b, 
         for (int nt = 0; nt < NT; nt++) s[m][nt] += s2[m][nt];
     }
     settle_all(s);
+    if (!kOwn) __builtin_amdgcn_s_setprio(0);
     if (masked) {
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
@@ -584,6 +587,7 @@ __device__ __forceinline__ bool attend(const AttnArgs& A, const Tile& X, int b, 
             ph[m / 2][nt][(m & 1) * 2 + i / 2] = a;
             pl[m / 2][nt][(m & 1) * 2 + i / 2] = e;
           }
+      if (!kOwn) __builtin_amdgcn_s_setprio(1);
       auto v_pair = [&](int d, int kk) {
         const u32x2 w0 = kOwn ? vf[kOwn ? d : 0][2 * kk] : v_frag(va, d, 2 * kk);
         const u32x2 w1 = kOwn ? vf[kOwn ? d : 0][2 * kk + 1] : v_frag(va, d, 2 * kk + 1);
@@ -625,6 +629,7 @@ __device__ __forceinline__ bool attend(const AttnArgs& A, const Tile& X, int b, 
           }
     }
     settle_all(acc);
+    if (!kOwn) __builtin_amdgcn_s_setprio(0);
   };
 
   // ---- the split's tiles ---------------------------------------------------------------------------
