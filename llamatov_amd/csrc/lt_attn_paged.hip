@@ -844,25 +844,25 @@ int form_kt(Form f, int hd, bool f16) {
   return f == kRows128 && hd <= 128 ? 64 : 32;
 }
 
-Plan make_plan(int T, int B, int nh, const PagedKv& C, bool f16, int max_q, int max_len, int window) {
+Plan plan_form(Form form, int T, int B, int nh, const PagedKv& C, bool f16, int max_len, int window) {
   Plan P;
   const int rep = nh / C.nkv;
-  if (max_q <= 0 || max_q > T) max_q = T;
-  const long long rows = (long long)max_q * rep;
-  const bool wide = C.hd > 128;
-  P.form = rows <= 16 ? kDecode16 : wide ? kRows128 : rows <= 32 ? kDecode32 : rows <= 64 ? kRows64 : kRows128;
-  P.tm = P.form == kDecode16 ? 16 : P.form == kDecode32 ? 32 : P.form == kRows64 || wide ? 64 : 128;
-  P.kt = form_kt(P.form, C.hd, f16);
+  P.form = form;
+  P.per_seq = form == kDecode16 || form == kDecode32;
+  P.tm = form == kDecode16 ? 16 : form == kDecode32 ? 32 : form == kRows64 || C.hd > 128 ? 64 : 128;
+  P.kt = form_kt(form, C.hd, f16);
   const int seqs = B < T ? B : T;
   const long long full = (long long)T * rep / P.tm;
-  P.per_seq = P.form == kDecode16 || P.form == kDecode32;
   P.tiles = P.per_seq ? B : (int)(full + seqs);
-  // splits: enough workgroups for the CUs (two a CU where registers allow it), of `least` keys at least
   const long long cap = (long long)C.stride << C.shift;
   long long len = max_len > 0 ? max_len : 4096;
   if (len > cap) len = cap;
+  // Splits: to as many workgroups as the CUs hold at once, of `least` keys at least.  Few rows (one workgroup a CU, its
+  // ring fills LDS): one token over 32768 at 32 / 64 / 43 splits (256, 512, 344 workgroups) 32 / 36 / 38 us.  Tiles of
+  // 128 rows (two a CU): four chunks over 6000 at 512 / 1024 / 1536 workgroups 171 / 186 / 224 us.
   const long long est = (full > seqs ? full : seqs) * C.nkv;
-  long long want = !P.per_seq ? (2 * kCus + est - 1) / est : est >= kCus ? 1 : kCus / est;
+  const long long resident = form == kRows64 ? kCus : 2 * kCus;
+  long long want = !P.per_seq ? (resident + est - 1) / est : est >= kCus ? 1 : kCus / est;
   if (want > kMaxSplits) want = kMaxSplits;
   const long long least = P.per_seq ? 256 : 128, unit = P.per_seq ? 128 : 64;   // unit: the key tiles of all groups
   P.most = (int)((len + least - 1) / least < want ? (len + least - 1) / least : want);
@@ -871,6 +871,28 @@ Plan make_plan(int T, int B, int nh, const PagedKv& C, bool f16, int max_q, int 
   if (chunk < least) chunk = least;
   P.chunk = (int)((chunk + unit - 1) / unit * unit);
   P.nsplit = (int)((len + P.chunk - 1) / P.chunk);
+  return P;
+}
+
+// Rows of a sequence's KV head, at most: to 16 a wave's own tile, four waves on different keys; to 32 two waves' (eight drafts
+// of 5 x 4 rows 14.7 us, with 32 rows a wave 17.5); past that workgroups that share their keys.  Of those, 64 rows with
+// 16 a wave make more workgroups and need fewer splits, 128 with 32 a wave read less of LDS a product, which pays once a
+// workgroup has kLongKeys keys to go through (64 / 128 rows: 2 x 500 tokens over 2000, 700 keys a workgroup, 54 / 87 us;
+// 4 x 509 over 6000, 3300 keys, 153 / 159; 512 over 14336, 3700 keys, 224 / 211; 2048 over 14336 864 / 792).  The fp32
+// instruction is slow enough for the narrow form throughout (2 x 500 over 2000 241 / 250).
+constexpr int kLongKeys = 3500;
+Plan make_plan(int T, int B, int nh, const PagedKv& C, bool f16, int max_q, int max_len, int window) {
+  if (max_q <= 0 || max_q > T) max_q = T;
+  const long long rows = (long long)max_q * (nh / C.nkv);
+  auto form = [&](Form f) { return plan_form(f, T, B, nh, C, f16, max_len, window); };
+  if (rows <= 16) return form(kDecode16);
+  if (C.hd > 128) return form(kRows128);
+  if (rows <= 32) return form(kDecode32);
+  if (rows <= 64 || !f16) return form(kRows64);
+  const Plan wide = form(kRows128);
+  if (wide.chunk >= kLongKeys) return wide;
+  Plan P = form(kRows64);
+  P.most = wide.most > P.most ? wide.most : P.most;   // another window may take the other form
   return P;
 }
 

@@ -169,16 +169,18 @@ def test_attention_windows(gpu, window, kv):
 
 def test_attention_split_windows(gpu):
     """Windows over long contexts: the workspace of the whole context serves every window."""
-    b = Batch(gpu, [5, 1], [3000, 2600], 8, 2, 64, 32, "f16", seed=21)
-    for window in (300, 700, 1000, 2047, 2999, 5000):
-        case(f"attention split window {window}")
-        b.check(window=window)
-    b.free()
+    for news, pasts in (([5, 1], [3000, 2600]), ([40, 17], [4500, 2600])):
+        b = Batch(gpu, news, pasts, 8, 2, 64, 32, "f16", seed=21)
+        for window in (300, 700, 1000, 2047, 2999, 5000):
+            case(f"attention split window {window} {news}")
+            b.check(window=window)
+        b.free()
 
 
 @pytest.mark.parametrize("kv", ["f16", "f32"])
 @pytest.mark.parametrize("news,pasts,max_len", [([1], [5000], None), ([5, 1, 2], [3000, 1, 900], None),
-                                                ([70], [2500], None), ([1, 1], [4097, 130], 1), ([40], [2000], 0)])
+                                                ([70], [2500], None), ([1, 1], [4097, 130], 1), ([40], [2000], 0),
+                                                ([90, 3], [3900, 100], None)])
 def test_attention_splits(gpu, news, pasts, max_len, kv):
     """Long contexts of few rows, and host bounds that are wrong or not known."""
     case(f"attention long {news} {pasts} {max_len} {kv}")
@@ -188,6 +190,17 @@ def test_attention_splits(gpu, news, pasts, max_len, kv):
     assert np.array_equal(first, again)      # no order of arrival in the result
     if max_len is None:
         b.check(max_q=1, max_len=100000)
+    b.free()
+
+
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("nh,nkv,hd", [(14, 2, 64), (8, 2, 128), (6, 1, 96), (4, 1, 40), (4, 2, 256)])
+def test_attention_long_chunks(gpu, nh, nkv, hd, kv):
+    """Many rows over contexts long enough for the widest tiles, with and without a window."""
+    b = Batch(gpu, [75, 1, 40], [3650, 17, 2000], nh, nkv, hd, 32, kv, seed=hd)
+    for window in (0, 3600, 700):
+        case(f"attention long chunks {nh}/{nkv}/{hd} {kv} window {window}")
+        b.check(window=window)
     b.free()
 
 
@@ -233,19 +246,19 @@ def test_attention_peaked_and_flat(gpu, kv):
 
 
 @pytest.mark.parametrize("kv", ["f16", "f32"])
-@pytest.mark.parametrize("n", [4, 20, 90])
-def test_attention_masked_infinities(gpu, n, kv):
+@pytest.mark.parametrize("n,past", [(4, 33), (20, 33), (90, 33), (90, 3800)])
+def test_attention_masked_infinities(gpu, n, past, kv):
     """A later token's K and V of infinities and NaN do not reach the rows before it; the rows that attend it follow
     the formula."""
-    case(f"attention masked infinities, chunk of {n}, {kv}")
-    at = 33 + n - 2
+    case(f"attention masked infinities, chunk of {n} over {past}, {kv}")
+    at = past + n - 2
 
     def spoil(b):
         b.V[0][at, 0, 3] = np.inf
         b.V[0][at, 1, 5] = np.nan
         b.V[0][at + 1, 0, 3] = -np.inf
         b.K[0][at + 1, 1] = np.nan
-    b = Batch(gpu, [n], [33], 8, 2, 64, 16, kv, seed=n, vals=spoil)
+    b = Batch(gpu, [n], [past], 8, 2, 64, 16, kv, seed=n, vals=spoil)
     got = b.attend().reshape(n, 2, 4, 64)
     with np.errstate(all="ignore"):
         exp, tol = b.expect()
@@ -266,11 +279,11 @@ def test_attention_masked_infinities(gpu, n, kv):
 
 
 @pytest.mark.parametrize("kv", ["f16", "f32"])
-@pytest.mark.parametrize("n", [1, 6, 40, 90])
-def test_attention_attended_infinities(gpu, n, kv):
+@pytest.mark.parametrize("n,past", [(1, 300), (6, 300), (40, 300), (90, 300), (90, 3700)])
+def test_attention_attended_infinities(gpu, n, past, kv):
     """Infinities among the values and keys that every row attends, deep inside the context: the formula's infinity, NaN
     where two of them cancel, nothing else touched; a key of -inf for positive queries has no weight."""
-    case(f"attention attended infinities, chunk of {n}, {kv}")
+    case(f"attention attended infinities, chunk of {n} over {past}, {kv}")
 
     def spoil(b):
         b.V[0][100, 0, 3] = np.inf
@@ -279,7 +292,7 @@ def test_attention_attended_infinities(gpu, n, kv):
         b.V[0][104, 1, 6] = np.nan
         b.K[0][200] = -np.inf
         b.V[0][200] = 1000.0
-    b = Batch(gpu, [n], [300], 8, 2, 64, 16, kv, seed=n, vals=spoil)
+    b = Batch(gpu, [n], [past], 8, 2, 64, 16, kv, seed=n, vals=spoil)
     b.q[:] = np.abs(b.q) + 0.25
     b.q[:, 1] = 0.5                                    # exact in few bits: the second term has nothing left
     b.dq.upload(b.q)

@@ -123,6 +123,22 @@ def test_workspace_sizes():
     assert a(1, 1, 4, desc(hd=12), 0, 0) == 0      # refused geometries have no size
 
 
+def test_workspace_serves_every_window():
+    """The size asked for without a window is enough with any (arithmetic of the launch plan)."""
+    need = _lib.raw("lt_attn_paged_workspace_size")
+    run = _lib.raw("lt_attn_paged")
+    for page, stride in ((16, 300), (64, 512)):
+        for f16 in (LT_KV_F16, LT_KV_F32):
+            for nh, nkv, hd in ((8, 2, 64), (32, 8, 128), (4, 1, 256)):
+                kv = PagedKvDesc(4096, 4096, 4, stride, 100, page, nkv, hd, f16)
+                for T in (1, 4, 9, 30, 100, 700, 3000):
+                    for L in (1, 300, 4000, 30000):
+                        n = need(T, 2, nh, kv, T, L)
+                        for window in (1, 100, 1000, 3499, 3600, 20000):
+                            rc = run(None, 16, nh * hd, T, 4, 4, 2, nh, kv, 16, 0.1, window, T, L, 16, n, None)
+                            assert rc == -1 and "null ctx" in _lib.last_error(), (T, L, window, _lib.last_error())
+
+
 class HostDevice:
     """Device memory as host byte arrays."""
     handle = None
