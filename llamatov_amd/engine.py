@@ -1954,6 +1954,121 @@ class BatchStepGraph:
             self.graph = ctypes.c_void_p()
 
 
+class PagedBatch:
+    """A model's forward pass over a batch of chunks on a paged cache, and the verification of drafts in them (no
+    reference counterpart): the linear layers of the batched prefill over all packed rows, RoPE + append and attention
+    through the cache's pages.  A chunk is a prompt's next part, or a token and the drafts after it; logits[r] belong to
+    packed row r.  Lengths stay on the device: advance() takes a chunk as it is, verify() as far as it is accepted."""
+
+    def __init__(self, model: ResidentModel, cache: PagedKVCache, max_rows: int):
+        cfg, D = model.cfg, model.dev
+        kv = cache.layers[0].desc
+        if len(cache.layers) != cfg.n_layers or (kv.nkv, kv.hd) != (cfg.n_head_kv, cfg.head_dim):
+            raise ValueError("PagedBatch: the cache is not of this model's geometry")
+        if "wgu_il" not in model.layers[0]:
+            raise ValueError("PagedBatch needs the fused gate|up layout (ResidentModel layouts 'fused' or 'both')")
+        if max_rows < 1:
+            raise ValueError(f"PagedBatch: max_rows={max_rows}")
+        model.prefill_tiles()
+        self.head = model.head_tiles()
+        self.model, self.cfg, self.cache, self.dev, self.max_rows = model, cfg, cache, D, int(max_rows)
+        T, E, F, B = self.max_rows, cfg.n_embd, cfg.n_ff, cache.max_seqs
+        kmax = max(E, F, cfg.q_dim)
+        self.toks, self.q_start = DevTensor.empty((T,), np.int32, D), DevTensor.zeros((B + 1,), np.int32, D)
+        self.x, self.xres = DevTensor.empty((T, E), np.float32, D), DevTensor.empty((T, E), np.float32, D)
+        self.qkv, self.att = DevTensor.empty((T, cfg.n_qkv), np.float32, D), DevTensor.empty((T, cfg.q_dim), np.float32, D)
+        self.v = DevTensor.empty((T, F), np.float32, D)
+        self.xq, self.xd = DevTensor.empty((T * kmax,), np.int8, D), DevTensor.empty((T * kmax // 32,), np.uint16, D)
+        self.logits = DevTensor.empty((T, cfg.vocab), np.float32, D)
+        self.out_tok, self.n_out = DevTensor.empty((T,), np.int32, D), DevTensor.empty((B,), np.int32, D)
+        self.err = DevTensor.zeros((1,), np.int32, D)
+        self.params = DevTensor.zeros((B, 32), np.uint8, D)      # lt_sample_params of each sequence: greedy
+        self.verify_ws = DevTensor.empty((max(verify_drafts_workspace_size(T, cfg.vocab, True), 16),), np.uint8, D)
+        self._attn_ws: DevTensor | None = None
+        self.rows: list[int] = [0] * B
+
+    def set_params(self, b: int, temperature: float, top_k: int = 40, top_p: float = 1.0, seed: int = 0) -> None:
+        """Sampling of sequence b (temperature 0: greedy), as DecodePlan.set_sampling."""
+        p = np.zeros(1, np.dtype([("temperature", "<f4"), ("top_k", "<i4"), ("top_p", "<f4"), ("reserved", "<i4"),
+                                  ("seed", "<u8"), ("counter", "<u8")]))
+        p["temperature"], p["top_k"], p["top_p"], p["seed"] = temperature, top_k, top_p, seed
+        self.dev.h2d(self.params.ptr + 32 * b, p.view(np.uint8))
+
+    def step(self, chunks) -> None:
+        """Run chunks[b], sequence b's next tokens (maybe none), through the model: their K and V rows after the
+        cached ones, their logits.  The cache's lengths are left for advance() or verify()."""
+        if len(chunks) != self.cache.max_seqs:
+            raise ValueError(f"{len(chunks)} chunks for a cache of {self.cache.max_seqs} sequences")
+        rows = [len(c) for c in chunks]
+        T = sum(rows)
+        if T > self.max_rows:
+            raise ValueError(f"{T} rows for a PagedBatch of {self.max_rows}")
+        if T == 0:
+            self.rows = rows
+            self.dev.h2d(self.q_start.ptr, np.zeros(len(rows) + 1, np.int32))
+            return
+        ends = [n + r for n, r in zip(self.cache.lengths(), rows)]
+        for b, end in enumerate(ends):
+            self.cache.reserve(b, end)
+        self.rows = rows
+        self.dev.h2d(self.q_start.ptr, np.cumsum([0] + rows).astype(np.int32))
+        self.dev.h2d(self.toks.ptr, np.asarray([int(t) for c in chunks for t in c], np.int32))
+        self._enqueue(T, max(rows), max(ends))
+
+    def _enqueue(self, T: int, max_q: int, max_len: int) -> None:
+        cfg, m, h = self.cfg, self.model, self.dev.handle
+        E, F, nh, QD, NQ = cfg.n_embd, cfg.n_ff, cfg.n_head, cfg.q_dim, cfg.n_qkv
+        eps, scale = ctypes.c_float(cfg.norm_eps), float(cfg.head_dim ** -0.5)
+        need = attn_paged_workspace_size(T, self.q_start.n - 1, nh, self.cache.layers[0], max_q, max_len)
+        if need and (self._attn_ws is None or self._attn_ws.nbytes < need):
+            if self._attn_ws is not None:
+                self.dev.sync()
+                self._attn_ws.free()
+            self._attn_ws = DevTensor.empty((need,), np.uint8, self.dev)
+        qkv, att = self.qkv.view(0, (T, NQ)), self.att.view(0, (T, QD))
+        xq, xd = self.xq.vp, self.xd.vp
+        call("lt_embed_q8_batch", h, m.tok_embd.t.vp, self.toks.vp, self.x.vp, T, E, cfg.vocab, self.err.vp)
+        for L, kv in zip(m.layers, self.cache.layers):
+            call("lt_rmsnorm_quant_bm", h, self.x.vp, L["attn_norm"].vp, xq, xd, T, E, eps)
+            call("lt_q8_gemm_t", h, L["wqkv_t"].t.vp, xq, xd, _vp(L["bqkv"]), None, qkv.vp, T, NQ, E)
+            rope_append_paged_into(qkv, qkv, self.q_start, self.cache.lens, nh, m.freqs, kv, self.err)
+            attn_paged_into(qkv, self.q_start, self.cache.lens, kv, nh, scale, att, max_q=max_q, max_len=max_len,
+                            ws=self._attn_ws, err=self.err)
+            call("lt_quant_q8_bm", h, att.vp, xq, xd, T, QD)
+            call("lt_q8_gemm_t", h, L["wo_t"].t.vp, xq, xd, None, self.x.vp, self.xres.vp, T, E, QD)
+            call("lt_rmsnorm_quant_bm", h, self.xres.vp, L["ffn_norm"].vp, xq, xd, T, E, eps)
+            call("lt_q8_gemm_silu_t", h, L["wgu_il_t"].t.vp, xq, xd, self.v.vp, T, F, E)
+            call("lt_quant_q8_bm", h, self.v.vp, xq, xd, T, F)
+            call("lt_q8_gemm_t", h, L["wdown_t"].t.vp, xq, xd, None, self.xres.vp, self.x.vp, T, E, F)
+        call("lt_rmsnorm_quant_bm", h, self.x.vp, m.output_norm.vp, xq, xd, T, E, eps)
+        call("lt_q8_gemm_t", h, self.head.t.vp, xq, xd, None, None, self.logits.vp, T, cfg.vocab, E)
+
+    def advance(self) -> None:
+        """The last step's rows stay in the cache."""
+        call("lt_len_add_rows", self.dev.handle, self.cache.lens.vp, self.q_start.vp, self.cache.max_seqs,
+             self.cache.max_pages * self.cache.page)
+
+    def verify(self, u: DevTensor | None = None, draft_logits: DevTensor | None = None) -> list[list[int]]:
+        """Verify the drafts of the last step (every token of a chunk after its first) under each sequence's sampling,
+        keep the accepted rows, and return each sequence's new tokens: the accepted drafts and the one after them."""
+        T = sum(self.rows)
+        if T == 0:
+            return [[] for _ in self.rows]
+        logits = self.logits.view(0, (T, self.cfg.vocab))
+        verify_drafts_into(logits, self.toks, self.q_start, u, self.params, self.out_tok, self.n_out, self.verify_ws,
+                           draft_logits=draft_logits, lens=self.cache.lens)
+        out, n = self.out_tok.to_host(), self.n_out.to_host()
+        at = np.cumsum([0] + self.rows)
+        return [[int(t) for t in out[at[b]:at[b] + n[b]]] for b in range(len(self.rows))]
+
+    def free(self) -> None:
+        self.dev.sync()
+        for t in (self.toks, self.q_start, self.x, self.xres, self.qkv, self.att, self.v, self.xq, self.xd, self.logits,
+                  self.out_tok, self.n_out, self.err, self.params, self.verify_ws, self._attn_ws):
+            if t is not None:
+                t.free()
+
+
 def batch_generate(model: ResidentModel, prompts, n_tokens: int, profile: Profile = PRODUCTION_PROFILE,
                    max_ctx: int | None = None, linear: str = "auto") -> list[list[int]]:
     """Greedy generation of n_tokens after each of len(prompts) prompts, decoded together:
