@@ -621,8 +621,8 @@ LT_API int lt_rope_append_paged(lt_ctx* ctx, const float* qkv, int row_stride, f
 
 /* Attention of the T rows (q: nh heads of hd, rows q_stride floats apart) over the paged cache: token i of
  * sequence b attends positions 0 .. len[b]+i, of them the last `window` where window > 0; the chunk's own
- * rows are in the cache already.  out [T][nh*hd] fp32 = softmax(scale q.k) v, with scores, statistics and
- * sums in fp32 or more.  What lies in masked places (any value, infinities and NaN among them) has no
+ * rows are in the cache already.  out [T][nh*hd] fp32 (not q's memory) = softmax(scale q.k) v, with scores,
+ * statistics and sums in fp32 or more.  What lies in masked places (any value, infinities and NaN among them) has no
  * effect.  A position in a page outside the pool reads as a row of zeros, and rows past the table's row
  * attend what the table holds; both set *err = 1 (device int, may be null).
  * max_q and max_len are the host's bounds on a sequence's rows and on len[b] plus them (0: not known); they

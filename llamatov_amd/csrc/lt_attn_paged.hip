@@ -27,9 +27,12 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 
 constexpr float kLog2e = 1.4426950408889634f;
-// P is held as 2^7 exp2(score - reference), the reference moved once a score passes it by 8: at most 2^15, and a weight
-// of 2^-32 of the largest still has a term
-constexpr float kPShift = 7.0f, kSlack = 8.0f;
+// P is held as 2^kPShift exp2(score - reference), the reference moved once a score passes it by kSlack.  For binary16
+// terms at most 2^15, and a weight of 2^-32 of the largest still has a term; in fp32 at most 1, so that values near the
+// type's largest do not overflow
+constexpr float kSlack = 8.0f;
+template <bool F16>
+constexpr float kPShift = F16 ? 7.0f : -kSlack;
 constexpr int kMaxSplits = 128, kCus = 256;
 
 __device__ const u32x4 g_zero16 = {0, 0, 0, 0};   // what a row without a page reads
@@ -236,7 +239,7 @@ __device__ __forceinline__ void rows_one_by_one(const AttnArgs& A, const Tile& X
 #pragma unroll
       for (int x = 32; x; x >>= 1) mt = fmaxf(mt, __shfl_xor(mt, x, 64));
       const float mn = fmaxf(m, mt), mu = mn == -__builtin_inff() ? 0.0f : mn;
-      const float a = __builtin_amdgcn_exp2f(m - mu), p = __builtin_amdgcn_exp2f(s - mu + kPShift);
+      const float a = __builtin_amdgcn_exp2f(m - mu), p = __builtin_amdgcn_exp2f(s - mu + kPShift<F16>);
       float zt = p;
 #pragma unroll
       for (int x = 32; x; x >>= 1) zt += __shfl_xor(zt, x, 64);
@@ -565,7 +568,7 @@ __device__ __forceinline__ bool attend(const AttnArgs& A, const Tile& X, int b, 
     }
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      const float bias = kPShift - (mref[nt] == -__builtin_inff() ? 0.0f : mref[nt]);
+      const float bias = kPShift<F16> - (mref[nt] == -__builtin_inff() ? 0.0f : mref[nt]);
 #pragma unroll
       for (int m = 0; m < MT; m++)
 #pragma unroll
@@ -773,7 +776,7 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(AttnArgs A, int tm, int
     t = r - q0;
     X = tile_of(A, q0, A.q_start[b + 1], A.len[b], (t * A.rep + (head - div_by(A.by_rep, head) * A.rep)) / tm, tm, kt);
   }
-  const bool on = b >= 0 && X.nact > 1;
+  const bool on = b >= 0 && X.rows > 0 && X.nact > 1;
   const size_t row = (size_t)r * A.nh + head, at = row * A.nsplit;
   float m = -__builtin_inff(), z = 0.0f;
   f32x4 o = {0, 0, 0, 0};

@@ -17,7 +17,7 @@ __global__ __launch_bounds__(256) void k_rope_append_paged(const float* __restri
   const int r = blockIdx.x, hd = C.hd, half = hd >> 1, nkv = C.nkv;
   const int b = seq_of_row(q_start, B, r);
   if (b < 0) return;
-  const int pos = len[b] + (r - q_start[b]);
+  const int pos = (int)((uint32_t)len[b] + (uint32_t)(r - q_start[b]));   // past 2^31: negative, no page
   const int pg = page_of(C, b, pos);
   if (pg < 0 && err && threadIdx.x == 0) *err = 1;
   for (int j = threadIdx.x; j < half; j += 256) lt_sincosf((float)pos * freqs[j], &s_sn[j], &s_cs[j]);

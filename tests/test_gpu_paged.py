@@ -246,6 +246,33 @@ def test_attention_peaked_and_flat(gpu, kv):
 
 
 @pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
+def test_attention_scales(gpu, scale, kv):
+    """A negative scale turns the order of the keys round, zero makes every weight the same."""
+    case(f"attention scale {scale} {kv}")
+    b = Batch(gpu, [3, 40], [700, 20], 4, 2, 64, 16, kv, seed=6)
+    b.scale = scale
+    got = b.attend()
+    k, b.scale = b.K, abs(scale)
+    b.K = [x * np.sign(scale).astype(x.dtype) for x in b.K]
+    exp, tol = b.expect()
+    assert np.all(np.abs(got - exp) <= tol)
+    b.free()
+
+
+@pytest.mark.parametrize("n", [2, 40])
+def test_attention_large_fp32_values(gpu, n):
+    """Values near the largest binary32: the result is a mean of them, and no step of the way is larger."""
+    case(f"attention large values, chunk of {n}")
+
+    def large(b):
+        b.V[0] *= np.float32(2.0 ** 115)              # to 2^117, 400 of them, and a weight of 2^-8 at most each step
+    b = Batch(gpu, [n], [400], 4, 2, 64, 16, "f32", seed=7, vals=large)
+    b.check()
+    b.free()
+
+
+@pytest.mark.parametrize("kv", ["f16", "f32"])
 @pytest.mark.parametrize("n,past", [(4, 33), (20, 33), (90, 33), (90, 3800)])
 def test_attention_masked_infinities(gpu, n, past, kv):
     """A later token's K and V of infinities and NaN do not reach the rows before it; the rows that attend it follow

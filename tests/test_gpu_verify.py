@@ -284,6 +284,16 @@ def test_verification_replayed(gpu):
         x.free()
 
 
+def test_verification_rows_behind_the_last_sequence(gpu):
+    case("verify rows behind")
+    rng = np.random.default_rng(10)
+    logits, dl, toks, start, u, params = batch(rng, 700, [3, 2, 4], SETTINGS, True)
+    start = start[:3]                                   # the last sequence's rows belong to nobody
+    out, n, _, _ = run(gpu, logits, dl, toks, start, u, params[:2])
+    eo, en = verify(logits[:5], dl[:5], toks[:5], start, u[:5], params[:2])
+    assert np.array_equal(n, en) and np.array_equal(out[:5], eo) and np.all(out[5:] == -9)
+
+
 def test_verification_no_rows(gpu):
     case("verify no rows")
     n = dr.DevTensor.from_host(np.full(2, -9, np.int32), gpu)
