@@ -768,6 +768,22 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(AttnArgs A, int tm, int
   const uint32_t item = blockIdx.x * (256 / per) + sub;   // T * nh < 2^31
   const int r = __builtin_amdgcn_readfirstlane(div_by(A.by_nh, (int)item));
   const int head = __builtin_amdgcn_readfirstlane((int)item) - r * A.nh;
+  const size_t row = (size_t)r * A.nh + head, at = row * A.nsplit;
+  // four splits of this group from s on; the first four are asked for before it is known how many took part
+  float ms[4], zs[4];
+  f32x4 x[4];
+  const bool mine = r < A.T && d < hd;
+  auto load = [&](int s) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int sj = s + j * groups;
+      const bool in = mine && sj < A.nsplit;
+      ms[j] = in ? A.ws.m[at + sj] : 0.0f;
+      zs[j] = in ? A.ws.z[at + sj] : 0.0f;
+      x[j] = in ? *(const f32x4*)(A.ws.o + (at + sj) * hd + d) : (f32x4){0, 0, 0, 0};
+    }
+  };
+  load(grp);
   const int b = r < A.T ? seq_of_row(A.q_start, A.B, r) : -1;
   Tile X = {};
   int t = 0;
@@ -777,33 +793,30 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(AttnArgs A, int tm, int
     X = tile_of(A, q0, A.q_start[b + 1], A.len[b], (t * A.rep + (head - div_by(A.by_rep, head) * A.rep)) / tm, tm, kt);
   }
   const bool on = b >= 0 && X.rows > 0 && X.nact > 1;
-  const size_t row = (size_t)r * A.nh + head, at = row * A.nsplit;
   float m = -__builtin_inff(), z = 0.0f;
   f32x4 o = {0, 0, 0, 0};
   if (on && d < hd) {
-    for (int s = grp; s < X.nact; s += 4 * groups) {
-      float ms[4], zs[4];
-      f32x4 x[4];
+    for (int s = grp; s < X.nact;) {
+      float mn = m;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const int sj = s + j * groups;
-        const bool in_range = sj < X.nact;
-        ms[j] = in_range ? A.ws.m[at + sj] : -__builtin_inff();
-        zs[j] = in_range ? A.ws.z[at + sj] : 0.0f;
-        x[j] = in_range ? *(const f32x4*)(A.ws.o + (at + sj) * hd + d) : (f32x4){0, 0, 0, 0};
+        if (s + j * groups >= X.nact) ms[j] = -__builtin_inff();
+        mn = fmaxf(mn, ms[j]);
       }
-      const float mn = fmaxf(fmaxf(m, fmaxf(ms[0], ms[1])), fmaxf(ms[2], ms[3]));
       const float a0 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
       z *= a0;
       o *= a0;
       m = mn;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
+        if (s + j * groups >= X.nact) continue;   // what lies there was not written
         const float a = ms[j] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ms[j] - mn);
         z = fmaf(zs[j], a, z);
 #pragma unroll
         for (int e = 0; e < 4; e++) o[e] = fmaf(x[j][e], a, o[e]);
       }
+      s += 4 * groups;
+      if (s < X.nact) load(s);
     }
   }
   *(f32x4*)(so + threadIdx.x * 4) = o;

@@ -211,6 +211,14 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
   __shared__ double s_px;
   __shared__ int s_n, s_count;
   const int row = blockIdx.x, t = threadIdx.x;
+  // the groups' maxima, asked for before it is known that the row takes part
+  uint32_t key[4];
+  bool live[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    live[j] = j * kSmThreads + t < A.groups;
+    key[j] = live[j] ? A.ws.top[(size_t)row * A.groups + j * kSmThreads + t] : 0u;
+  }
   int b, draft;
   const float* l = vf_row(A, row, &b, &draft);
   if (!l) return;
@@ -221,14 +229,6 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
   uint32_t bound = 0u;
   int count;
   {
-    uint32_t key[4];
-    bool live[4];
-    const uint32_t* top = A.ws.top + (size_t)row * A.groups;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      live[j] = j * kSmThreads + t < A.groups;
-      key[j] = live[j] ? top[j * kSmThreads + t] : 0u;
-    }
     if (t == 0) s_count = 0;
     if (A.groups > kc) {
       int rem;
