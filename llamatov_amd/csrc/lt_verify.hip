@@ -201,6 +201,16 @@ __device__ __forceinline__ u64 sort_stage(u64 x, int size) {
   return (x > y) == first ? x : y;   // the pairs are distinct, padding apart
 }
 
+// The stages of one block size whose partners lie in the same wave.
+__device__ __forceinline__ u64 sort_wave(u64 x, int size) {
+  if (size >= 64) x = sort_stage<32>(x, size);
+  if (size >= 32) x = sort_stage<16>(x, size);
+  if (size >= 16) x = sort_stage<8>(x, size);
+  if (size >= 8) x = sort_stage<4>(x, size);
+  if (size >= 4) x = sort_stage<2>(x, size);
+  return sort_stage<1>(x, size);
+}
+
 template <bool VEC>
 __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
   __shared__ SmShared S;
@@ -209,7 +219,7 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
   __shared__ double s_sum[kSmWaves];
   __shared__ double s_c[kSmMaxK];
   __shared__ double s_px;
-  __shared__ int s_n, s_count;
+  __shared__ int s_n, s_count, s_groups;
   const int row = blockIdx.x, t = threadIdx.x;
   // the groups' maxima, asked for before it is known that the row takes part
   uint32_t key[4];
@@ -229,21 +239,31 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
   uint32_t bound = 0u;
   int count;
   {
-    if (t == 0) s_count = 0;
+    if (t == 0) s_count = s_groups = 0;
     if (A.groups > kc) {
       int rem;
       bound = radix_select<4, 2>(key, live, kc, S, &rem);
 #pragma unroll
       for (int j = 0; j < 4; j++) live[j] = live[j] && key[j] >= bound;
     }
+    u64 m[4];
     int sel = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++) sel += live[j];
-    int o = block_excl_scan(sel, S, &count);
+    for (int j = 0; j < 4; j++) {
+      m[j] = __ballot(live[j]);
+      sel += (int)__popcll(m[j]);
+    }
+    __syncthreads();   // the counters are zero
+    int o = 0;
+    if ((t & 63) == 0 && sel) o = atomicAdd(&s_groups, sel);
+    o = __builtin_amdgcn_readfirstlane(o);
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (live[j]) s_grp[o++] = j * kSmThreads + t;
+    for (int j = 0; j < 4; j++) {
+      if (live[j]) s_grp[o + (int)__popcll(m[j] & ((1ull << (t & 63)) - 1))] = j * kSmThreads + t;
+      o += (int)__popcll(m[j]);
+    }
     __syncthreads();
+    count = s_groups;
   }
   // their logits at or above the bound, in any order (the sort settles it)
   auto gather = [&](u64 least) {
@@ -295,8 +315,46 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
     __syncthreads();
     M = gather(prefix);
   }
+  // the weight of this thread's candidate, of k
+  auto weight = [&](u64 pair, float l0, int k) {
+    if (t >= k) return 0.0;
+    if (k == 1) return 1.0;
+    return exp(((double)key_logit((uint32_t)(pair >> 32)) - (double)l0) / (double)P->temperature);
+  };
   int P2 = 1;
   u64 x = 0ull;   // padding: below every candidate
+  if (M <= 64) {
+    // one wave holds them all: no more waits of the workgroup
+    if (t >= 64) return;
+    x = t < M ? s_key[t] : 0ull;
+    for (int size = 2; size <= 64; size <<= 1) x = sort_wave(x, size);
+    const float l0 = key_logit((uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)));
+    const int k = __builtin_isfinite(l0) ? kc : 1;
+    const double w = weight(x, l0, k);
+    double c = w;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double y = __shfl_up(c, o, 64);
+      if (t >= o) c += y;
+    }
+    const float topp = P->top_p;
+    const u64 cut = topp < 1.0f ? __ballot(t < k && c >= (double)topp * __shfl(c, k - 1, 64)) : 0ull;
+    const int n = cut ? __builtin_ctzll(cut) + 1 : k;
+    const double total = __shfl(c, n - 1, 64);
+    const int id = (int)~(uint32_t)x;
+    const double p = w / total;
+    if (t < n) {
+      A.ws.p[(size_t)row * kSmMaxK + t] = p;
+      A.ws.id[(size_t)row * kSmMaxK + t] = id;
+    }
+    const u64 at = __ballot(t < n && id == draft);
+    const double px = at ? __shfl(p, __builtin_ctzll(at), 64) : 0.0;
+    if (t == 0) {
+      A.ws.n[row] = n;
+      A.ws.px[row] = px;
+    }
+    return;
+  }
   if (M <= kSmThreads) {
     while (P2 < M) P2 <<= 1;
     if (t < M) x = s_key[t];
@@ -347,7 +405,7 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
     __syncthreads();
   }
   // bitonic network, larger first, one key a thread; partners in other waves trade through LDS, in two halves in turn
-  if (P2 > 64 || t < 64) {
+  {
     int half = 0;
     for (int size = 2; size <= P2; size <<= 1) {
       for (int stride = size >> 1; stride >= 64; stride >>= 1) {
@@ -358,12 +416,7 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
         const bool first = ((t & size) == 0) == ((t & stride) == 0);
         x = (x > y) == first ? x : y;
       }
-      if (size >= 64) x = sort_stage<32>(x, size);
-      if (size >= 32) x = sort_stage<16>(x, size);
-      if (size >= 16) x = sort_stage<8>(x, size);
-      if (size >= 8) x = sort_stage<4>(x, size);
-      if (size >= 4) x = sort_stage<2>(x, size);
-      x = sort_stage<1>(x, size);
+      x = sort_wave(x, size);
     }
   }
   __syncthreads();
@@ -374,9 +427,7 @@ __global__ __launch_bounds__(kSmThreads) void k_verify_rows(VfArgs A) {
   __syncthreads();
   const float l0 = key_logit((uint32_t)(s_key[0] >> 32));
   const int k = __builtin_isfinite(l0) ? kc : 1;
-  const double w = t >= k ? 0.0
-                   : k == 1 ? 1.0
-                            : exp(((double)key_logit((uint32_t)(x >> 32)) - (double)l0) / (double)P->temperature);
+  const double w = weight(x, l0, k);
   double total;
   const double c = scan_f64(w, s_sum, &total);
   if (t == 0) s_n = k;
