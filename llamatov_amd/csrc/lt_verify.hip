@@ -20,6 +20,10 @@
 // whose maxima are not either; little more than k logits are read again, sorted, and turned into the distribution and
 // the probability of the row's draft.  The k-th maximum's leading 16 bits are bound enough.  (3) k_verify_seqs, one
 // workgroup a sequence: the first draft not accepted, and the last token.
+//
+// Measured at V = 151936, top_k 40: 64 sequences of up to 4 drafts with a drafter's logits 30.6 + 15.0 + 6.5 us (193 MB in
+// the first, 6.3 TB/s: bound by memory), one sequence 5.0 + 9.8 + 4.7 (latency); 72 rows of 128256 with 1024 candidates
+// 8.6 + 25.2 + 4.8.
 #include <type_traits>
 
 #include "lt_internal.h"
@@ -34,7 +38,7 @@ namespace {
 constexpr int kVfMaxV = 262144;
 constexpr int kVfGroups = 4 * kSmThreads;           // groups of a row at most: four a thread
 constexpr int kVfCand = 4 * kSmThreads;             // logits not below the bound that LDS holds
-constexpr int kVfSpan = 8192;                       // logits of a workgroup of k_verify_maxima
+constexpr int kVfSpan = 8192;                       // logits of a workgroup of k_verify_maxima: 32 a thread, all asked for at once
 typedef unsigned long long u64;
 
 struct VfWs {
@@ -569,7 +573,8 @@ __global__ __launch_bounds__(kSeqThreads) void k_verify_seqs(VfArgs A) {
   }
 }
 
-// Neighbours of a group: at most kVfGroups groups a row, and many more than the 1024 that a row may select.
+// Neighbours of a group: at most kVfGroups groups a row (four a thread), and as many as that allows, so that a group that
+// is selected brings few logits with it.
 int vf_group(int V) { return V <= 4 * kVfGroups ? 4 : V <= 16 * kVfGroups ? 16 : V <= 32 * kVfGroups ? 32 : 64; }
 
 int vf_groups(int V) { return (V + vf_group(V) - 1) / vf_group(V); }
