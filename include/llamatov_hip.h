@@ -610,8 +610,8 @@ typedef struct lt_paged_kv {
 } lt_paged_kv;
 
 /* RoPE and the append of the T rows of q|k|v (row_stride floats apart): the rotated q heads to q_out
- * (rows q_stride floats apart; q_out may be qkv itself with q_stride == row_stride), the rotated k and
- * the v to the cache.  The values of lt_rope_append_batch, bit for bit (the angle is the binary32 product
+ * (rows q_stride floats apart; q_out may be qkv itself with q_stride == row_stride, and overlaps it in no
+ * other way), the rotated k and the v to the cache.  The values of lt_rope_append_batch, bit for bit (the angle is the binary32 product
  * of the position and freqs[j]); qkv's own k and v are left as they are.  A row whose position lies past
  * the table's row, or in a page outside the pool, is not stored and sets *err = 1 (device int, may be
  * null); its q is written all the same. */

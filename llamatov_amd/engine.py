@@ -492,12 +492,23 @@ class PagedKVCache:
         self.lens.free()
 
 
+def _check_batch(what: str, q_start: DevTensor, lens: DevTensor, kv: PagedKV) -> int:
+    """Sequences of a packed batch, each with a length and a table row."""
+    B = q_start.n - 1
+    if B > lens.n or B > kv.table.shape[0]:
+        raise ValueError(f"{what}: {B} sequences, {lens.n} lengths, {kv.table.shape[0]} table rows")
+    return B
+
+
 def rope_append_paged_into(qkv: DevTensor, q_out: DevTensor, q_start: DevTensor, lens: DevTensor, nh: int,
                            freqs: DevTensor, kv: PagedKV, err: DevTensor | None = None) -> DevTensor:
     """RoPE of q|k|v rows [T, width] at each sequence's positions, rotated q into q_out [T, ...], k and v into
     the paged cache (lt_rope_append_paged)."""
+    B = _check_batch("rope_append_paged_into", q_start, lens, kv)
+    if q_out.shape[0] < qkv.shape[0] or 2 * freqs.n < kv.desc.hd:
+        raise ValueError(f"rope_append_paged_into: q_out {q_out.shape}, {freqs.n} frequencies for {qkv.shape} rows")
     call("lt_rope_append_paged", qkv.dev.handle, qkv.ptr, qkv.shape[1], q_out.ptr, q_out.shape[1], qkv.shape[0],
-         q_start.ptr, lens.ptr, q_start.n - 1, nh, freqs.ptr, kv.desc, _vp(err))
+         q_start.ptr, lens.ptr, B, nh, freqs.ptr, kv.desc, _vp(err))
     return q_out
 
 
@@ -509,7 +520,10 @@ def attn_paged_into(q: DevTensor, q_start: DevTensor, lens: DevTensor, kv: Paged
                     out: DevTensor, max_q: int = 0, max_len: int = 0, window: int = 0, ws: DevTensor | None = None,
                     err: DevTensor | None = None) -> DevTensor:
     """Attention of the rows of q [T, at least nh*hd] over the paged cache into out [T, nh*hd] (lt_attn_paged)."""
-    call("lt_attn_paged", q.dev.handle, q.ptr, q.shape[1], q.shape[0], q_start.ptr, lens.ptr, q_start.n - 1, nh, kv.desc,
+    B = _check_batch("attn_paged_into", q_start, lens, kv)
+    if out.n < q.shape[0] * nh * kv.desc.hd:
+        raise ValueError(f"attn_paged_into: out {out.shape} for {q.shape[0]} rows of {nh} heads of {kv.desc.hd}")
+    call("lt_attn_paged", q.dev.handle, q.ptr, q.shape[1], q.shape[0], q_start.ptr, lens.ptr, B, nh, kv.desc,
          out.ptr, scale, window, max_q, max_len, ws.ptr if ws is not None else None,
          ws.nbytes if ws is not None else 0, _vp(err))
     return out
@@ -524,8 +538,13 @@ def verify_drafts_into(logits: DevTensor, toks: DevTensor, q_start: DevTensor, u
                        lens: DevTensor | None = None) -> DevTensor:
     """Accept or reject the drafts of a batch of chunks against logits [T, V] and draw each sequence's next token
     (lt_verify_drafts); u None: the numbers come from each sequence's sampling state."""
+    (T, V), B = logits.shape, q_start.n - 1
+    if min(toks.n, out_tok.n, T if u is None else u.n) < T or (draft_logits is not None and draft_logits.shape != (T, V)):
+        raise ValueError(f"verify_drafts_into: tokens, numbers or draft logits do not match {T} rows of {V} logits")
+    if min(n_out.n, B if lens is None else lens.n) < B or params.nbytes < 32 * B:
+        raise ValueError(f"verify_drafts_into: counts, lengths or sampling states do not match {B} sequences")
     call("lt_verify_drafts", logits.dev.handle, logits.ptr, _vp(draft_logits), toks.ptr, q_start.ptr, _vp(u), params.ptr,
-         q_start.n - 1, logits.shape[0], logits.shape[1], out_tok.ptr, n_out.ptr, _vp(lens), ws.ptr, ws.nbytes)
+         B, T, V, out_tok.ptr, n_out.ptr, _vp(lens), ws.ptr, ws.nbytes)
     return out_tok
 
 

@@ -214,3 +214,36 @@ def test_descriptor_refusals():
         dr.PagedKVCache(1, 4, 24, 2, 8, 1, 4, dev=dev)
     with pytest.raises(ValueError):
         dr.PagedKVCache(1, 4, 16, 2, 8, 0, 4, dev=dev)
+
+
+def test_python_entries_check_shapes():
+    """Sequences without a length or a table row, outputs that are too small: refused before the library is called."""
+    dev = HostDevice()
+
+    def t(*shape, dt=np.float32):
+        return dr.DevTensor.empty(shape, dt, dev)
+
+    kv = dr.PagedKV(t(4, 2, 16, 8), t(4, 2, 16, 8), dr.DevTensor.zeros((2, 4), np.int32, dev), LT_KV_F32)
+    q, out, fr = t(6, 64), t(6, 32), t(4)
+    start3, start4, lens = t(3, dt=np.int32), t(4, dt=np.int32), t(2, dt=np.int32)
+    with pytest.raises(_lib.LtError, match="null ctx"):
+        dr.attn_paged_into(q, start3, lens, kv, 4, 0.3, out)
+    for args in ((q, start4, lens, kv, 4, 0.3, out), (q, start3, t(1, dt=np.int32), kv, 4, 0.3, out),
+                 (q, start3, lens, kv, 4, 0.3, t(5, 32))):
+        with pytest.raises(ValueError):
+            dr.attn_paged_into(*args)
+    with pytest.raises(_lib.LtError, match="null ctx"):
+        dr.rope_append_paged_into(q, out, start3, lens, 4, fr, kv)
+    for args in ((q, out, start4, lens, 4, fr, kv), (q, t(5, 32), start3, lens, 4, fr, kv), (q, out, start3, lens, 4, t(3), kv)):
+        with pytest.raises(ValueError):
+            dr.rope_append_paged_into(*args)
+    n = dr.verify_drafts_workspace_size(6, 100, True)
+    i32 = np.int32
+    good = dict(logits=t(6, 100), toks=t(6, dt=i32), q_start=start3, u=t(6), params=t(64, dt=np.uint8), out_tok=t(6, dt=i32),
+                n_out=t(2, dt=i32), ws=t(n, dt=np.uint8), draft_logits=t(6, 100), lens=lens)
+    with pytest.raises(_lib.LtError, match="null ctx"):
+        dr.verify_drafts_into(**good)
+    for bad in (dict(toks=t(5, dt=i32)), dict(u=t(5)), dict(out_tok=t(5, dt=i32)), dict(n_out=t(1, dt=i32)),
+                dict(params=t(63, dt=np.uint8)), dict(draft_logits=t(6, 99)), dict(lens=t(1, dt=i32))):
+        with pytest.raises(ValueError):
+            dr.verify_drafts_into(**{**good, **bad})
