@@ -878,20 +878,39 @@ Plan plan_form(Form form, int T, int B, int nh, const PagedKv& C, bool f16, int 
   const long long cap = (long long)C.stride << C.shift;
   long long len = max_len > 0 ? max_len : 4096;
   if (len > cap) len = cap;
-  // Splits: to as many workgroups as the CUs hold at once, of `least` keys at least.  Few rows (one workgroup a CU, its
-  // ring fills LDS): one token over 32768 at 32 / 64 / 43 splits (256, 512, 344 workgroups) 32 / 36 / 38 us.  Tiles of
-  // 128 rows (two a CU): four chunks over 6000 at 512 / 1024 / 1536 workgroups 171 / 186 / 224 us.
-  const long long est = (full > seqs ? full : seqs) * C.nkv;
-  const long long resident = form == kRows64 ? kCus : 2 * kCus;
-  long long want = !P.per_seq ? (resident + est - 1) / est : est >= kCus ? 1 : kCus / est;
-  if (want > kMaxSplits) want = kMaxSplits;
-  const long long least = P.per_seq ? 256 : 128, unit = P.per_seq ? 128 : 64;   // unit: the key tiles of all groups
-  P.most = (int)((len + least - 1) / least < want ? (len + least - 1) / least : want);
-  if (window > 0 && len > (long long)window + P.tm / rep + 2) len = (long long)window + P.tm / rep + 2;   // of one tile
-  long long chunk = (len + want - 1) / want;
-  if (chunk < least) chunk = least;
-  P.chunk = (int)((chunk + unit - 1) / unit * unit);
-  P.nsplit = (int)((len + P.chunk - 1) / P.chunk);
+  const long long est = (full > seqs ? full : seqs) * C.nkv;       // workgroups of one split
+  const long long least = P.per_seq ? 256 : 128, unit = P.per_seq ? 128 : 64;   // keys; unit: the key tiles of all groups
+  long long span = len;                                             // keys of one tile's rows
+  if (window > 0 && span > (long long)window + P.tm / rep + 2) span = (long long)window + P.tm / rep + 2;
+  auto set = [&](long long want) {
+    long long chunk = (span + want - 1) / want;
+    if (chunk < least) chunk = least;
+    P.chunk = (int)((chunk + unit - 1) / unit * unit);
+    P.nsplit = (int)((span + P.chunk - 1) / P.chunk);
+  };
+  // Splits.  Tiles of 128 rows, to two workgroups a CU, which is what registers allow: four chunks over 6000 at 512 / 1024 /
+  // 1536 workgroups 171 / 186 / 224 us.  Tiles of 64 rows, where the CUs are not all taken, to two a CU (11 x 96 tokens over
+  // 3640 at 3 / 1 splits 37 / 44 us); where they are, the join costs more than it gives (8 x 64 over 500 at 2 / 1 splits 29
+  // / 20).
+  long long most = form == kRows128 ? (2 * kCus + est - 1) / est : form == kRows64 && est >= kCus ? 1 : 2 * kCus / est;
+  most = most < 1 ? 1 : most > kMaxSplits ? kMaxSplits : most;
+  set(most);
+  if (P.per_seq) {
+    // Few rows: one workgroup a CU (its ring fills LDS), so that what counts is rounds of workgroups.  In keys: those of a
+    // split and about 200 for a workgroup's beginning and end each round, and 300 for the join.  One token over 32768
+    // at 32 / 64 / 43 splits (256, 512, 344 workgroups) 32 / 36 / 38 us.
+    long long best = 0, pick = 1;
+    for (long long w = 1; w <= most; w++) {
+      set(w);
+      const long long cost = (est * P.nsplit + kCus - 1) / kCus * (P.chunk + 200) + (P.nsplit > 1 ? 300 : 0);
+      if (w == 1 || cost < best) {
+        best = cost;
+        pick = w;
+      }
+    }
+    set(pick);
+  }
+  P.most = (int)((len + least - 1) / least < most ? (len + least - 1) / least : most);
   return P;
 }
 
