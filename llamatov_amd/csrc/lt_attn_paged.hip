@@ -907,6 +907,7 @@ Plan plan_form(Form form, int T, int B, int nh, const PagedKv& C, bool f16, int 
         best = cost;
         pick = w;
       }
+      if (P.chunk <= least) break;   // no shorter split
     }
     set(pick);
   }

@@ -414,7 +414,7 @@ class PagedKV:
     """One layer's paged cache as the launches take it: K and V pools [n_pages][nkv][page][hd] and the
     table of page ids, int32 [sequences][pages a sequence] (lt_paged_kv; no reference counterpart, its
     DeviceKVCache holds one sequence).  The tensors stay the caller's."""
-    __slots__ = ("k", "v", "table", "desc")
+    __slots__ = ("k", "v", "table", "desc", "ref")
 
     def __init__(self, k: DevTensor, v: DevTensor, table: DevTensor, kv_dtype: int):
         if len(k.shape) != 4 or k.shape != v.shape:
@@ -427,6 +427,7 @@ class PagedKV:
         n_pages, nkv, page, hd = k.shape
         self.k, self.v, self.table = k, v, table
         self.desc = _lib.PagedKvDesc(k.ptr, v.ptr, table.ptr, table.shape[1], n_pages, page, nkv, hd, kv_dtype)
+        self.ref = ctypes.byref(self.desc)
 
 
 class PagedKVCache:
@@ -508,12 +509,12 @@ def rope_append_paged_into(qkv: DevTensor, q_out: DevTensor, q_start: DevTensor,
     if q_out.shape[0] < qkv.shape[0] or 2 * freqs.n < kv.desc.hd:
         raise ValueError(f"rope_append_paged_into: q_out {q_out.shape}, {freqs.n} frequencies for {qkv.shape} rows")
     call("lt_rope_append_paged", qkv.dev.handle, qkv.ptr, qkv.shape[1], q_out.ptr, q_out.shape[1], qkv.shape[0],
-         q_start.ptr, lens.ptr, B, nh, freqs.ptr, kv.desc, _vp(err))
+         q_start.ptr, lens.ptr, B, nh, freqs.ptr, kv.ref, err.ptr if err is not None else None)
     return q_out
 
 
 def attn_paged_workspace_size(T: int, B: int, nh: int, kv: PagedKV, max_q: int = 0, max_len: int = 0) -> int:
-    return int(_lib.raw("lt_attn_paged_workspace_size")(T, B, nh, kv.desc, max_q, max_len))
+    return int(_lib.raw("lt_attn_paged_workspace_size")(T, B, nh, kv.ref, max_q, max_len))
 
 
 def attn_paged_into(q: DevTensor, q_start: DevTensor, lens: DevTensor, kv: PagedKV, nh: int, scale: float,
@@ -523,9 +524,9 @@ def attn_paged_into(q: DevTensor, q_start: DevTensor, lens: DevTensor, kv: Paged
     B = _check_batch("attn_paged_into", q_start, lens, kv)
     if out.n < q.shape[0] * nh * kv.desc.hd:
         raise ValueError(f"attn_paged_into: out {out.shape} for {q.shape[0]} rows of {nh} heads of {kv.desc.hd}")
-    call("lt_attn_paged", q.dev.handle, q.ptr, q.shape[1], q.shape[0], q_start.ptr, lens.ptr, B, nh, kv.desc,
+    call("lt_attn_paged", q.dev.handle, q.ptr, q.shape[1], q.shape[0], q_start.ptr, lens.ptr, B, nh, kv.ref,
          out.ptr, scale, window, max_q, max_len, ws.ptr if ws is not None else None,
-         ws.nbytes if ws is not None else 0, _vp(err))
+         ws.nbytes if ws is not None else 0, err.ptr if err is not None else None)
     return out
 
 
