@@ -14,7 +14,7 @@
 // the fp32 instruction would take.  An fp32 cache runs on the 16x16x4 fp32 instruction.
 //
 // Measured (fp16, 32 query heads over 8 of 128): one token over 32768 positions 23.8 us and the join 4.8 (134 MB, 5.6 TB/s;
-// bound by memory); 64 sequences of 512 to 4096 positions 124 us (614 MB, 4.95 TB/s); 2048 tokens over 14336 797 to 822 us (515
+// bound by memory); 64 sequences of 512 to 4096 positions 124 us (614 MB, 4.95 TB/s); 2048 tokens over 14336 797 to 852 us (515
 // GFLOP, 1.26 PFLOP/s of the two-term products; matrix pipes busy 62% of the time at 1.93 GHz, vector instructions 47%); a
 // short context 4.9 us (latency).  fp32, 14 heads over 2 of 64, 866 rows with a window of 512: 29.6 us and the join 9.2.
 #include "lt_paged.h"
