@@ -649,8 +649,8 @@ LT_API int lt_len_add_rows(lt_ctx* ctx, int* len, const int* q_start, int B, int
  * the first candidate in rank order whose running sum exceeds u times the whole.  u [T] device, in [0, 1);
  * null: u of row i of the sequence is Philox4x32-10's with counter params[b].counter + i (as lt_sample's),
  * and the counter advances by the sequence's rows.  Weights and sums are binary64.
- * out_tok [T]: a sequence's n_out[b] tokens from its first row on, then -1; n_out [B] (0 for a sequence
- * without rows).  len (may be null): len[b] += n_out[b], the chunk's rows that stay in the cache.
+ * out_tok [T] (not toks' memory): a sequence's n_out[b] tokens from its first row on, then -1; n_out [B]
+ * (0 for a sequence without rows).  len (may be null): len[b] += n_out[b], the chunk's rows that stay in the cache.
  * T <= 32767, V <= 262144.  ws holds lt_verify_drafts_workspace_size(T, V, draft_logits != NULL) bytes,
  * 8-byte aligned (0: the sizes are refused, or T is 0). */
 LT_API int lt_verify_drafts(lt_ctx* ctx, const float* logits, const float* draft_logits, const int* toks,

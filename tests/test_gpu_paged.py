@@ -623,3 +623,38 @@ def test_len_add_rows(gpu):
     assert np.array_equal(d.to_host(), np.minimum(ln + add, 52))
     d.free()
     s.free()
+
+
+def test_two_contexts_at_once(gpu):
+    """Calls of two contexts in flight together, each with its own workspace, give what they give alone."""
+    case("two contexts")
+    other = dr.Device(0)
+    batches = [Batch(d, [5, 1, 40], [1500, 3000, 90], 8, 2, 128, 16, kv, seed=s)
+               for d, kv, s in ((gpu, "f16", 1), (other, "f32", 2))]
+    alone = [b.attend() for b in batches]
+    ws = []
+    for b in batches:
+        n = dr.attn_paged_workspace_size(b.rows, 3, b.nh, b.kv, 40, 3001)
+        ws.append(dr.DevTensor.empty((max(n, 16),), np.uint8, b.gpu))
+        b.out.upload(np.full((b.rows, b.nh * b.hd), -7.0, np.float32))
+    for _ in range(20):
+        for b, w in zip(batches, ws):
+            dr.attn_paged_into(b.dq, b.ds, b.dl, b.kv, b.nh, b.scale, b.out, max_q=40, max_len=3001, ws=w)
+    for b, a in zip(batches, alone):
+        assert np.array_equal(b.out.to_host(), a)
+    for b, w in zip(batches, ws):
+        w.free()
+        b.free()
+    call("lt_free_ctx", other.handle)
+
+
+def test_shared_prefix_pages(gpu):
+    """Two sequences whose first pages are the same ones."""
+    case("shared pages")
+    b = Batch(gpu, [3, 3], [64, 64], 4, 2, 64, 16, "f16", seed=3)
+    t = b.table.copy()
+    t[1, :4] = t[0, :4]
+    b.dt.upload(t)
+    b.K[1][:64], b.V[1][:64] = b.K[0][:64], b.V[0][:64]
+    b.check()
+    b.free()
