@@ -855,6 +855,7 @@ struct Plan {
   int tm, kt;        // rows of a tile, keys of a key tile
   bool per_seq;      // a workgroup a sequence: all of its rows are one tile if max_q is right
   int tiles;         // workgroups along the batch
+  bool halves;       // workgroups of half the waves, two a CU
   int chunk, nsplit;
   int most;          // splits of any window: what the workspace is sized for
 };
@@ -911,6 +912,10 @@ Plan plan_form(Form form, int T, int B, int nh, const PagedKv& C, bool f16, int 
     }
     set(pick);
   }
+  // Up to 32 rows, four groups of waves a workgroup while each workgroup has a CU of its own, else two, so that one
+  // workgroup's products go beside another's waits (four / two: 8 x 5 tokens over 700 14.4 / 15.1 us, one of 5 over 30000 26.8
+  // / 28.5; 64 x 5 over 4096 148 / 129, 20 x 8 over 5727 81 / 67)
+  P.halves = form == kDecode32 && est * P.nsplit > kCus;
   P.most = (int)((len + least - 1) / least < most ? (len + least - 1) / least : most);
   return P;
 }
@@ -949,7 +954,10 @@ int launch(lt_ctx* ctx, const AttnArgs& A, const Plan& P) {
     case kDecode16:
       return go(k_attn_paged<HDP, 1, 1, KW, KT, F16, 1, true>, 64 * KW, Cfg<HDP, 1, 1, KW, KT, F16>::kLds);
     case kDecode32:
-      if constexpr (HDP <= 128) return go(k_attn_paged<HDP, 1, 2, 4, KT, F16, 1, true>, 512, Cfg<HDP, 1, 2, 4, KT, F16>::kLds);
+      if constexpr (HDP <= 128) {
+        if (P.halves) return go(k_attn_paged<HDP, 1, 2, 2, KT, F16, 1, true>, 256, Cfg<HDP, 1, 2, 2, KT, F16>::kLds);
+        return go(k_attn_paged<HDP, 1, 2, 4, KT, F16, 1, true>, 512, Cfg<HDP, 1, 2, 4, KT, F16>::kLds);
+      }
       break;
     case kRows64:
       if constexpr (HDP <= 128) return go(k_attn_paged<HDP, 1, 4, 2, KT, F16, 1, false>, 512, Cfg<HDP, 1, 4, 2, KT, F16>::kLds);

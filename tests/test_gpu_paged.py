@@ -215,6 +215,18 @@ def test_attention_large_batch(gpu):
     b.free()
 
 
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+def test_attention_many_drafts(gpu, kv):
+    """More workgroups of up to 32 rows than CUs, with and without splits."""
+    rng = np.random.default_rng(5)
+    for B, ctx in ((70, 150), (35, 900)):
+        case(f"attention {B} chunks of drafts over up to {ctx} {kv}")
+        news = [int(v) for v in rng.integers(1, 9, B)]
+        b = Batch(gpu, news, [int(v) for v in rng.integers(0, ctx, B)], 16, 4, 64, 16, kv, seed=B)
+        b.check(max_q=8)
+        b.free()
+
+
 def test_attention_strides(gpu):
     """q rows that are not 16-byte aligned, and rows behind the last sequence."""
     for extra in (1, 3, 8, 130):
