@@ -9,9 +9,9 @@ namespace {
 // k_rope_append_batch's arithmetic (the same q rows and cache values) with row r the token r - q_start[b] of
 // sequence b, at position len[b] + that, and its K and V rows at the page the table gives.  One workgroup a token takes
 // the hd / 2 sines and cosines (binary64) once for all heads.  Bound by memory: 1960 tokens of 48 heads of 128 move 69 MB in
-// 14.1 us (4.9 TB/s); one token 2.7 us.
+// 14.1 us (4.9 TB/s); one token 2.7 us.  qkv may be q_out, so neither pointer is __restrict__.
 template <bool kF16>
-__global__ __launch_bounds__(256) void k_rope_append_paged(const float* __restrict__ qkv, int row_stride, float* q_out,
+__global__ __launch_bounds__(256) void k_rope_append_paged(const float* qkv, int row_stride, float* q_out,
                                                            int q_stride, const int* __restrict__ q_start,
                                                            const int* __restrict__ len, int B, int nh,
                                                            const float* __restrict__ freqs, PagedKv C, int* err) {

@@ -614,7 +614,7 @@ size_t lt_verify_drafts_workspace_size(int T, int V, int drafter) {
 int lt_verify_drafts(lt_ctx* ctx, const float* logits, const float* draft_logits, const int* toks,
                      const int* q_start, const float* u, lt_sample_params* params, int B, int T, int V,
                      int* out_tok, int* n_out, int* len, void* ws, size_t ws_bytes) {
-  LT_REQUIRE(logits && toks && q_start && params && out_tok && n_out && ws, "lt_verify_drafts: null argument");
+  LT_REQUIRE(logits && toks && q_start && params && out_tok && n_out && (ws || T == 0), "lt_verify_drafts: null argument");
   LT_REQUIRE(B > 0 && B <= 65535 && vf_sizes(T, V), "lt_verify_drafts: B=%d (1 .. 65535) T=%d (0 .. 32767) V=%d (1 .. %d)",
              B, T, V, kVfMaxV);
   LT_REQUIRE(lt_aligned(params, 8) && lt_aligned(ws, 8) && lt_aligned(logits, 4) && lt_aligned(draft_logits, 4),

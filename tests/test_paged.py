@@ -103,6 +103,7 @@ def test_verification_refusals():
     refused(verify(dl=0, u=0), "null ctx")
     need = _lib.raw("lt_verify_drafts_workspace_size")(4, 100, 1)
     assert verify(n=need - 1) == -3
+    refused(verify(T=0, ws=0, n=0), "null ctx")     # no rows need no workspace
     refused(verify(n=need), "null ctx")
 
 
