@@ -455,6 +455,7 @@ class PagedKVCache:
 
     def reserve(self, b: int, positions: int) -> None:
         """Pages for sequence b's first `positions` positions; its table row on the device follows."""
+        self._check_seq(b)
         need = -(-int(positions) // self.page)
         more = need - len(self.pages[b])
         if need > self.max_pages:
@@ -468,10 +469,15 @@ class PagedKVCache:
 
     def release(self, b: int) -> None:
         """Sequence b's pages go back to the pool; its length becomes 0."""
+        self._check_seq(b)
         self.free_pages += self.pages[b][::-1]
         self.pages[b] = []
         self._push_row(b)
         self.dev.h2d(self.lens.ptr + 4 * b, np.zeros(1, np.int32))
+
+    def _check_seq(self, b: int) -> None:
+        if not 0 <= b < self.max_seqs:
+            raise ValueError(f"sequence {b} of a cache of {self.max_seqs}")
 
     def _push_row(self, b: int) -> None:
         row = np.full(self.max_pages, -1, np.int32)
@@ -2003,12 +2009,16 @@ class PagedBatch:
         self.out_tok, self.n_out = DevTensor.empty((T,), np.int32, D), DevTensor.empty((B,), np.int32, D)
         self.err = DevTensor.zeros((1,), np.int32, D)
         self.params = DevTensor.zeros((B, 32), np.uint8, D)      # lt_sample_params of each sequence: greedy
-        self.verify_ws = DevTensor.empty((max(verify_drafts_workspace_size(T, cfg.vocab, True), 16),), np.uint8, D)
         self._attn_ws: DevTensor | None = None
+        self._verify_ws: DevTensor | None = None
         self.rows: list[int] = [0] * B
+        self.open = False               # a step whose rows advance() or verify() has not counted yet
 
     def set_params(self, b: int, temperature: float, top_k: int = 40, top_p: float = 1.0, seed: int = 0) -> None:
         """Sampling of sequence b (temperature 0: greedy), as DecodePlan.set_sampling."""
+        self.cache._check_seq(b)
+        if not 1 <= int(top_k) <= LT_SAMPLE_MAX_K:
+            raise ValueError(f"top_k={top_k}: 1 .. {LT_SAMPLE_MAX_K}")
         p = np.zeros(1, np.dtype([("temperature", "<f4"), ("top_k", "<i4"), ("top_p", "<f4"), ("reserved", "<i4"),
                                   ("seed", "<u8"), ("counter", "<u8")]))
         p["temperature"], p["top_k"], p["top_p"], p["seed"] = temperature, top_k, top_p, seed
@@ -2023,28 +2033,46 @@ class PagedBatch:
         T = sum(rows)
         if T > self.max_rows:
             raise ValueError(f"{T} rows for a PagedBatch of {self.max_rows}")
+        toks = [int(t) for c in chunks for t in c]
+        if T and not 0 <= min(toks) <= max(toks) < self.cfg.vocab:
+            raise ValueError(f"a token outside the vocabulary of {self.cfg.vocab}")
         if T == 0:
-            self.rows = rows
+            self.rows, self.open = rows, True
             self.dev.h2d(self.q_start.ptr, np.zeros(len(rows) + 1, np.int32))
             return
         ends = [n + r for n, r in zip(self.cache.lengths(), rows)]
         for b, end in enumerate(ends):
             self.cache.reserve(b, end)
-        self.rows = rows
+        self.rows, self.open = rows, False
         self.dev.h2d(self.q_start.ptr, np.cumsum([0] + rows).astype(np.int32))
-        self.dev.h2d(self.toks.ptr, np.asarray([int(t) for c in chunks for t in c], np.int32))
+        self.dev.h2d(self.toks.ptr, np.asarray(toks, np.int32))
         self._enqueue(T, max(rows), max(ends))
+        self.open = True
+
+    def error(self) -> int:
+        """The device error word: 0 = none, 1 = a position outside the cache's pages (lengths set past what is
+        reserved)."""
+        return int(self.err.to_host()[0])
+
+    def _grown(self, ws: DevTensor | None, need: int) -> DevTensor | None:
+        if need and (ws is None or ws.nbytes < need):
+            if ws is not None:
+                self.dev.sync()
+                ws.free()
+            return DevTensor.empty((need,), np.uint8, self.dev)
+        return ws
+
+    def _count_rows(self, what: str) -> None:
+        if not self.open:
+            raise RuntimeError(f"PagedBatch.{what}: no step whose rows are not counted yet")
+        self.open = False
 
     def _enqueue(self, T: int, max_q: int, max_len: int) -> None:
         cfg, m, h = self.cfg, self.model, self.dev.handle
         E, F, nh, QD, NQ = cfg.n_embd, cfg.n_ff, cfg.n_head, cfg.q_dim, cfg.n_qkv
         eps, scale = ctypes.c_float(cfg.norm_eps), float(cfg.head_dim ** -0.5)
         need = attn_paged_workspace_size(T, self.q_start.n - 1, nh, self.cache.layers[0], max_q, max_len)
-        if need and (self._attn_ws is None or self._attn_ws.nbytes < need):
-            if self._attn_ws is not None:
-                self.dev.sync()
-                self._attn_ws.free()
-            self._attn_ws = DevTensor.empty((need,), np.uint8, self.dev)
+        self._attn_ws = self._grown(self._attn_ws, need)
         qkv, att = self.qkv.view(0, (T, NQ)), self.att.view(0, (T, QD))
         xq, xd = self.xq.vp, self.xd.vp
         call("lt_embed_q8_batch", h, m.tok_embd.t.vp, self.toks.vp, self.x.vp, T, E, cfg.vocab, self.err.vp)
@@ -2064,7 +2092,8 @@ class PagedBatch:
         call("lt_q8_gemm_t", h, self.head.t.vp, xq, xd, None, None, self.logits.vp, T, cfg.vocab, E)
 
     def advance(self) -> None:
-        """The last step's rows stay in the cache."""
+        """The last step's rows stay in the cache.  Either this or verify() once a step."""
+        self._count_rows("advance")
         call("lt_len_add_rows", self.dev.handle, self.cache.lens.vp, self.q_start.vp, self.cache.max_seqs,
              self.cache.max_pages * self.cache.page)
 
@@ -2072,10 +2101,17 @@ class PagedBatch:
         """Verify the drafts of the last step (every token of a chunk after its first) under each sequence's sampling,
         keep the accepted rows, and return each sequence's new tokens: the accepted drafts and the one after them."""
         T = sum(self.rows)
+        if T and draft_logits is not None and draft_logits.shape != (T, self.cfg.vocab):
+            raise ValueError(f"PagedBatch.verify: draft logits {draft_logits.shape} for {T} rows")
+        if T and u is not None and u.n < T:
+            raise ValueError(f"PagedBatch.verify: {u.n} numbers for {T} rows")
+        self._count_rows("verify")
         if T == 0:
             return [[] for _ in self.rows]
+        need = verify_drafts_workspace_size(T, self.cfg.vocab, draft_logits is not None)
+        self._verify_ws = self._grown(self._verify_ws, max(need, 16))
         logits = self.logits.view(0, (T, self.cfg.vocab))
-        verify_drafts_into(logits, self.toks, self.q_start, u, self.params, self.out_tok, self.n_out, self.verify_ws,
+        verify_drafts_into(logits, self.toks, self.q_start, u, self.params, self.out_tok, self.n_out, self._verify_ws,
                            draft_logits=draft_logits, lens=self.cache.lens)
         out, n = self.out_tok.to_host(), self.n_out.to_host()
         at = np.cumsum([0] + self.rows)
@@ -2084,7 +2120,7 @@ class PagedBatch:
     def free(self) -> None:
         self.dev.sync()
         for t in (self.toks, self.q_start, self.x, self.xres, self.qkv, self.att, self.v, self.xq, self.xd, self.logits,
-                  self.out_tok, self.n_out, self.err, self.params, self.verify_ws, self._attn_ws):
+                  self.out_tok, self.n_out, self.err, self.params, self._verify_ws, self._attn_ws):
             if t is not None:
                 t.free()
 

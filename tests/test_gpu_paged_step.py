@@ -142,3 +142,62 @@ def test_paged_batch_refusals(gpu, tiny):
     assert cache.pages == [[]]
     pb.free()
     cache.free()
+
+
+def test_paged_batch_counts_a_step_once(gpu, tiny):
+    """Rows are counted by one advance() or verify() a step; tokens, sequences and sampling settings are checked before."""
+    m, prompts = tiny
+    case("PagedBatch calls out of order")
+    c = m.cfg
+    cache = dr.PagedKVCache(c.n_layers, 4, 8, c.n_head_kv, c.head_dim, 2, 4, dev=gpu)
+    pb = dr.PagedBatch(m, cache, 8)
+    for call in (pb.advance, pb.verify):
+        with pytest.raises(RuntimeError):
+            call()
+    pb.step([prompts[0][:3], []])
+    pb.advance()
+    for call in (pb.advance, pb.verify):
+        with pytest.raises(RuntimeError):
+            call()
+    assert cache.lengths() == [3, 0]
+    for bad in (-1, c.vocab):
+        with pytest.raises(ValueError, match="vocabulary"):
+            pb.step([[1, bad], []])
+    for b, k in ((-1, 40), (2, 40), (0, 0), (0, 1025)):
+        with pytest.raises(ValueError):
+            pb.set_params(b, 0.8, top_k=k)
+    pb.step([[], prompts[1][:2]])
+    with pytest.raises(ValueError, match="numbers"):
+        pb.verify(u=dr.DevTensor.zeros((1,), np.float32, gpu))
+    got = pb.verify()
+    assert got[0] == [] and 1 <= len(got[1]) <= 2 and cache.lengths() == [3, len(got[1])] and pb.error() == 0
+    with pytest.raises(RuntimeError):
+        pb.verify()
+    pb.free()
+    cache.free()
+
+
+def test_paged_batch_verifies_with_a_drafter_after_none(gpu, tiny):
+    """The verification's workspace grows with what a step needs."""
+    m, prompts = tiny
+    case("PagedBatch verification, without and with a drafter's logits")
+    c = m.cfg
+    cache = dr.PagedKVCache(c.n_layers, 8, 8, c.n_head_kv, c.head_dim, 1, 8, dev=gpu)
+    pb = dr.PagedBatch(m, cache, 8)
+    pb.step([prompts[0]])
+    pb.advance()
+    pb.step([[1]])
+    assert len(pb.verify()[0]) == 1
+    pb.step([[2, 3, 4]])
+    logits = pb.logits.to_host()[:3]
+    best = logits.argmax(1)
+    pb.step([[2, int(best[0]), 4]])              # the first draft is the greedy token
+    logits = pb.logits.to_host()[:3]
+    draft = np.zeros_like(logits)
+    draft[0, best[0]] = 1.0
+    draft[1, 4] = 1.0
+    got = pb.verify(draft_logits=dr.DevTensor.from_host(draft, gpu))[0]
+    second = int(logits[1].argmax())
+    assert got == [int(best[0]), second] + ([int(logits[2].argmax())] if second == 4 else [])
+    pb.free()
+    cache.free()

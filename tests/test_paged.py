@@ -248,3 +248,14 @@ def test_python_entries_check_shapes():
                 dict(params=t(63, dt=np.uint8)), dict(draft_logits=t(6, 99)), dict(lens=t(1, dt=i32))):
         with pytest.raises(ValueError):
             dr.verify_drafts_into(**{**good, **bad})
+
+
+def test_page_account_takes_only_its_sequences():
+    """A sequence number outside the cache would address device memory before or behind the table and the lengths."""
+    c = dr.PagedKVCache(1, 4, 16, 2, 8, max_seqs=2, max_pages=2, kv_dtype=LT_KV_F32, dev=HostDevice())
+    for b in (-1, 2):
+        with pytest.raises(ValueError, match="cache of 2"):
+            c.reserve(b, 1)
+        with pytest.raises(ValueError, match="cache of 2"):
+            c.release(b)
+    assert c.pages == [[], []] and len(c.free_pages) == 4
