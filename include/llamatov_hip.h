@@ -652,7 +652,7 @@ LT_API int lt_len_add_rows(lt_ctx* ctx, int* len, const int* q_start, int B, int
  * out_tok [T] (not toks' memory): a sequence's n_out[b] tokens from its first row on, then -1; n_out [B]
  * (0 for a sequence without rows).  len (may be null): len[b] += n_out[b], the chunk's rows that stay in the cache.
  * T <= 32767, V <= 262144.  ws holds lt_verify_drafts_workspace_size(T, V, draft_logits != NULL) bytes,
- * 8-byte aligned (0: the sizes are refused, or T is 0). */
+ * 8-byte aligned (0: the sizes are refused, or T is 0 and ws may be null). */
 LT_API int lt_verify_drafts(lt_ctx* ctx, const float* logits, const float* draft_logits, const int* toks,
                             const int* q_start, const float* u, lt_sample_params* params, int B, int T, int V,
                             int* out_tok, int* n_out, int* len, void* ws, size_t ws_bytes);
